@@ -1,4 +1,5 @@
-"""ctypes binding of ``libglm_b200.so`` (the C ABI declared in ``include/glm_b200.h``).
+"""ctypes binding of ``libglm_b200.so`` (the C ABI declared in ``include/glm_b200.h``
+and ``include/glm_matrix_b200.h``).
 
 Every function here takes raw device pointers (integers) and sizes, calls
 the library and raises :class:`GlmbError` on a non-zero status.  The
@@ -32,6 +33,8 @@ GRAD_WRITE_YHAT = 0x2
 GRAD_Y_ZERO = 0x4
 GRAD_LOGISTIC = 0x8
 
+STEP_NESTEROV = 0x1
+
 #: the eleven element types of the reference mains, by C-ABI suffix
 REFERENCE_SUFFIXES = ("f16", "f32", "f64", "i8", "i16", "i32", "i64", "u8", "u16", "u32", "u64")
 #: every element type of predict / gradient / loss: the reference's eleven and bfloat16
@@ -39,6 +42,8 @@ SUFFIXES = REFERENCE_SUFFIXES + ("bf16",)
 FLOATING = ("f32", "f64")
 #: 16-bit types with the sharded entry points (partial, finalize, peer exchange) but no fit
 HALF16 = ("f16", "bf16")
+#: element types of the whole-matrix operators (glm_matrix_b200.h)
+MATRIX = ("f32", "f16", "bf16")
 
 
 class GlmbError(RuntimeError):
@@ -141,6 +146,31 @@ def _declare(L: ctypes.CDLL) -> None:
         getattr(L, name).restype = _INT
 
 
+def _declare_matrix(L: ctypes.CDLL) -> None:
+    L.glmm_q4_codes_bytes.argtypes = [_I64, _I64, _I64]
+    L.glmm_q4_codes_bytes.restype = _I64
+    L.glmm_q4_scales_count.argtypes = [_I64, _I64, _I64, _INT]
+    L.glmm_q4_scales_count.restype = _I64
+    for s in MATRIX:
+        sig = {
+            "glmm_orthogonalize": [_P, _P, _I64, _I64, _I64, _P, _INT, _P, _SZ, _P],
+            "glmm_orthogonal_step": [_P, _P, _P, _I64, _I64, _I64, _D, _D, _D, _D, _U32, _P, _INT, _P, _SZ, _P],
+            "glmm_quantize_q4": [_P, _P, _P, _I64, _I64, _I64, _INT, _P],
+            "glmm_dequantize_q4": [_P, _P, _P, _I64, _I64, _I64, _INT, _P],
+            "glmm_predict_q4": [_P, _P, _P, _P, _I64, _I64, _I64, _I64, _INT, _P, _SZ, _P],
+        }
+        for name, args in sig.items():
+            f = getattr(L, f"{name}_{s}")
+            f.argtypes = args
+            f.restype = _INT
+        f = getattr(L, f"glmm_orthogonal_workspace_size_{s}")
+        f.argtypes = [_I64, _I64, _I64]
+        f.restype = _SZ
+        f = getattr(L, f"glmm_predict_q4_workspace_size_{s}")
+        f.argtypes = [_I64, _I64, _I64, _I64, _INT]
+        f.restype = _SZ
+
+
 def lib() -> ctypes.CDLL:
     """The loaded library; raises if it has not been built."""
     global _lib
@@ -151,6 +181,7 @@ def lib() -> ctypes.CDLL:
                 "(the GLM path has no host fallback)")
         _lib = ctypes.CDLL(LIB_PATH)
         _declare(_lib)
+        _declare_matrix(_lib)
     return _lib
 
 
@@ -202,4 +233,14 @@ def exported_symbols() -> list[str]:
     names += ["glmb_mg_create", "glmb_mg_destroy", "glmb_mg_size", "glmb_mg_stream", "glmb_mg_synchronize"]
     for s in FLOATING:
         names += [f"glmb_mg_gradient_{s}", f"glmb_mg_fit_elastic_net_{s}"]
+    return names
+
+
+def matrix_symbols() -> list[str]:
+    """Every entry point declared in include/glm_matrix_b200.h (for the load test)."""
+    names = ["glmm_q4_codes_bytes", "glmm_q4_scales_count"]
+    for s in MATRIX:
+        names += [f"glmm_{op}_{s}" for op in
+                  ("orthogonal_workspace_size", "orthogonalize", "orthogonal_step", "quantize_q4", "dequantize_q4",
+                   "predict_q4_workspace_size", "predict_q4")]
     return names

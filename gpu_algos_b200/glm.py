@@ -10,8 +10,18 @@ torch shapes ``[sheet, row, col]``:
 
 Every call launches asynchronously on ``stream`` (default: torch's current
 stream) and goes to ``libglm_b200.so``; there is no host or torch fallback.
+
+The whole-matrix operators at the end (:func:`orthogonalize`,
+:func:`orthogonal_step`, :func:`quantize_q4`, :func:`dequantize_q4`,
+:func:`predict_q4`; float32, float16 and bfloat16) also launch on the tensors'
+own device where that is not the current one, and allocate what they return
+on ``stream``.
 """
 from __future__ import annotations
+
+import contextlib
+import ctypes
+import math
 
 import torch
 
@@ -233,3 +243,187 @@ def fit_elastic_net(X, Y, lambda1: float, lambda2: float, n_power: int = 20, n_i
               ntasks, nobs, float(lambda1), float(lambda2), int(n_power), int(n_iter),
               int(seed) & (2**64 - 1), ws_ptr, ws_bytes, _stream(stream))
     return beta, lipschitz
+
+
+# ---- whole-matrix operators: orthogonalised updates, models in 4 bits ----------------
+
+MATRIX_DTYPES = (torch.float32, torch.float16, torch.bfloat16)
+
+
+def _matrix_suffix(dtype) -> str:
+    if dtype not in MATRIX_DTYPES:
+        raise ValueError(f"dtype {dtype} is not one of float32, float16, bfloat16")
+    return SUFFIX[dtype]
+
+
+@contextlib.contextmanager
+def _launch_on(device, stream):
+    """The tensors' device and the call's stream are current (allocations
+    included) while the library is called; yields the stream's handle."""
+    if stream is not None and stream.device != device:
+        raise ValueError(f"stream is on {stream.device}, the tensors are on {device}")
+    with torch.cuda.device(device):
+        with torch.cuda.stream(stream) if stream is not None else contextlib.nullcontext():
+            yield torch.cuda.current_stream(device).cuda_stream
+
+
+def _need_on(t: torch.Tensor, name: str, shape, dtype, device) -> None:
+    _need(t, name, shape, dtype)
+    if t.device != device:
+        raise ValueError(f"{name} is on {t.device}, expected {device}")
+
+
+def _workspace(workspace, device):
+    if workspace is None:
+        return None, 0
+    if workspace.device != device:
+        raise ValueError(f"workspace is on {workspace.device}, expected {device}")
+    if not workspace.is_contiguous():
+        raise ValueError("workspace must be contiguous")
+    return workspace.data_ptr(), workspace.numel() * workspace.element_size()
+
+
+def _model_dims(M: torch.Tensor, name: str):
+    if M.dim() != 3:
+        raise ValueError(f"{name} has shape {tuple(M.shape)}, expected (ntasks, ntargets, nfeatures)")
+    return M.shape
+
+
+def _coefficients(coefficients, steps: int):
+    """A host array of 3*steps doubles, or None for the library's own."""
+    if coefficients is None:
+        return None
+    rows = list(coefficients)
+    if len(rows) == 3 and all(isinstance(v, (int, float)) for v in rows):
+        rows = [rows] * steps
+    if len(rows) != steps or any(len(r) != 3 for r in rows):
+        raise ValueError(f"coefficients must be one (a, b, c) or {steps} of them")
+    return (ctypes.c_double * (3 * steps))(*[float(v) for r in rows for v in r])
+
+
+def orthogonal_workspace_bytes(dtype, nf: int, nt: int, ntasks: int) -> int:
+    """Workspace of :func:`orthogonalize` and :func:`orthogonal_step`."""
+    return int(getattr(capi.lib(), f"glmm_orthogonal_workspace_size_{_matrix_suffix(dtype)}")(nf, nt, ntasks))
+
+
+def orthogonalize(G, steps: int = 5, coefficients=None, out=None, workspace=None, stream=None):
+    """Newton-Schulz orthogonalisation of every task's matrix of ``G``
+    ``(ntasks, ntargets, nfeatures)``: X = G/|G|_F (zero stays zero), then
+    ``steps`` times X <- aX + (bA + cA^2)X with A = X X^T on the shorter side.
+
+    ``coefficients``: one (a, b, c) or one per step, by default (3.4445,
+    -4.7750, 2.0315), which brings the singular values near 1 in five steps.
+    ``out`` may be ``G``."""
+    sfx = _matrix_suffix(G.dtype)
+    ntasks, nt, nf = _model_dims(G, "G")
+    _need(G, "G", G.shape, G.dtype)
+    coef = _coefficients(coefficients, int(steps))
+    with _launch_on(G.device, stream) as s:
+        if out is None:
+            out = torch.empty_like(G)
+        _need_on(out, "out", G.shape, G.dtype, G.device)
+        ws_ptr, ws_bytes = _workspace(workspace, G.device)
+        capi.call(f"glmm_orthogonalize_{sfx}", _ptr(G), _ptr(out), nf, nt, ntasks, coef, int(steps), ws_ptr,
+                  ws_bytes, s)
+    return out
+
+
+def orthogonal_step(M, grad, momentum, lr: float, mu: float = 0.95, nesterov: bool = True,
+                    weight_decay: float = 0.0, scale: float | None = None, steps: int = 5, coefficients=None,
+                    workspace=None, stream=None):
+    """One update of the model ``M`` by its orthogonalised momentum, in place:
+
+        momentum <- mu*momentum + grad             (float32, M's shape)
+        U = grad + mu*momentum if nesterov else momentum
+        M <- (1 - lr*weight_decay)*M - lr*scale*orthogonalize(U)
+
+    ``grad`` has M's type (as :func:`gradient` returns it); ``scale`` is
+    sqrt(max(1, ntargets/nfeatures)) by default.  Returns ``M``."""
+    sfx = _matrix_suffix(M.dtype)
+    ntasks, nt, nf = _model_dims(M, "M")
+    _need(M, "M", M.shape, M.dtype)
+    _need_on(grad, "grad", M.shape, M.dtype, M.device)
+    _need_on(momentum, "momentum", M.shape, torch.float32, M.device)
+    if scale is None:
+        scale = math.sqrt(max(1.0, nt / nf)) if nf > 0 else 1.0
+    coef = _coefficients(coefficients, int(steps))
+    with _launch_on(M.device, stream) as s:
+        ws_ptr, ws_bytes = _workspace(workspace, M.device)
+        capi.call(f"glmm_orthogonal_step_{sfx}", _ptr(M), _ptr(grad), _ptr(momentum), nf, nt, ntasks, float(lr),
+                  float(mu), float(weight_decay), float(scale), capi.STEP_NESTEROV if nesterov else 0, coef,
+                  int(steps), ws_ptr, ws_bytes, s)
+    return M
+
+
+class Q4Model:
+    """A model in 4 bits: codes and one scale per target and group of
+    features, in the library's layout (``glm_matrix_b200.h``).  Made by
+    :func:`quantize_q4`; ``shape`` is ``(ntasks, ntargets, nfeatures)``."""
+
+    def __init__(self, shape, dtype, group: int, device):
+        ntasks, nt, nf = self.shape = tuple(int(v) for v in shape)
+        self.dtype, self.group = dtype, int(group)
+        _matrix_suffix(dtype)
+        if self.group not in (64, 128):
+            raise ValueError(f"group is {group}, expected 64 or 128")
+        L = capi.lib()
+        self.codes = torch.empty(L.glmm_q4_codes_bytes(nf, nt, ntasks), dtype=torch.uint8, device=device)
+        self.scales = torch.empty(L.glmm_q4_scales_count(nf, nt, ntasks, self.group), dtype=dtype, device=device)
+
+    @property
+    def device(self):
+        return self.codes.device
+
+
+def quantize_q4(M, group: int = 128, out=None, stream=None) -> Q4Model:
+    """``M`` in 4 bits: per target and group of 64 or 128 features a scale
+    s = max|w|/7 (rounded to M's type) and codes q = w/s rounded to the nearest
+    of -7..7, ties to even.  ``out``: a Q4Model of the same shape to overwrite."""
+    sfx = _matrix_suffix(M.dtype)
+    ntasks, nt, nf = _model_dims(M, "M")
+    _need(M, "M", M.shape, M.dtype)
+    with _launch_on(M.device, stream) as s:
+        if out is None:
+            out = Q4Model(M.shape, M.dtype, group, M.device)
+        if (out.shape, out.dtype, out.group, out.device) != (tuple(M.shape), M.dtype, group, M.device):
+            raise ValueError("out was made for another shape, dtype, group or device")
+        capi.call(f"glmm_quantize_q4_{sfx}", _ptr(M), _ptr(out.codes), _ptr(out.scales), nf, nt, ntasks, out.group, s)
+    return out
+
+
+def dequantize_q4(model: Q4Model, out=None, stream=None):
+    """The weights q*s of a :class:`Q4Model`, rounded to its dtype."""
+    ntasks, nt, nf = model.shape
+    with _launch_on(model.device, stream) as s:
+        if out is None:
+            out = torch.empty(model.shape, dtype=model.dtype, device=model.device)
+        _need_on(out, "out", model.shape, model.dtype, model.device)
+        capi.call(f"glmm_dequantize_q4_{SUFFIX[model.dtype]}", _ptr(model.codes), _ptr(model.scales), _ptr(out), nf,
+                  nt, ntasks, model.group, s)
+    return out
+
+
+def predict_q4_workspace_bytes(dtype, nf: int, nt: int, ntasks: int, nobs: int, group: int) -> int:
+    """Workspace of :func:`predict_q4`."""
+    return int(getattr(capi.lib(), f"glmm_predict_q4_workspace_size_{_matrix_suffix(dtype)}")(nf, nt, ntasks, nobs,
+                                                                                            int(group)))
+
+
+def predict_q4(X, model: Q4Model, out=None, workspace=None, stream=None):
+    """:func:`predict` from a :class:`Q4Model`: Yhat[obs, task, t] = sum_f
+    q[task, t, f]*s X[obs, task, f], from one observation to many; the products
+    are those of the exact weights q*s, sums are float32."""
+    sfx = _matrix_suffix(model.dtype)
+    ntasks, nt, nf = model.shape
+    if X.dim() != 3:
+        raise ValueError(f"X has shape {tuple(X.shape)}, expected (nobs, ntasks, nfeatures)")
+    nobs = X.shape[0]
+    _need_on(X, "X", (nobs, ntasks, nf), model.dtype, model.device)
+    with _launch_on(model.device, stream) as s:
+        if out is None:
+            out = torch.empty((nobs, ntasks, nt), dtype=X.dtype, device=X.device)
+        _need_on(out, "out", (nobs, ntasks, nt), X.dtype, X.device)
+        ws_ptr, ws_bytes = _workspace(workspace, X.device)
+        capi.call(f"glmm_predict_q4_{sfx}", _ptr(X), _ptr(model.codes), _ptr(model.scales), _ptr(out), nf, nt,
+                  ntasks, nobs, model.group, ws_ptr, ws_bytes, s)
+    return out
