@@ -56,14 +56,13 @@
 // status word, skips its remaining work, waits (bounded) for its copies and
 // MMAs in flight, meets its peer at the final cluster barrier, frees its
 // TMEM and exits, and the reduction kernel turns the status into NaN.
-#include <cuda.h>
-#include <cudaTypedefs.h>
 
 #include <algorithm>
 #include <mutex>
 
 #include "glm_common.cuh"
 #include "glm_dense.cuh"
+#include "glm_tc.cuh"
 
 namespace glmb {
 
@@ -92,7 +91,6 @@ constexpr int kATileBytes = kBM * kBK * 4;  // 16 KB
 constexpr int kBTileBytes = kBNHalf * kBK * 4;  // 16 KB
 constexpr int kAtomBytes = 32 * kBK * 4;    // MN-major: 32 M/N elements x kBK K-rows
 constexpr int kStageBytes = 2 * kATileBytes + 2 * kBTileBytes;
-constexpr long long kWaitCycles = 4ll << 30;  // ~2 s at 1.9 GHz
 constexpr uint32_t kReadyArrivals = 2 * kConvWarps;  // converter warps of both CTAs
 constexpr uint32_t kDrainArrivals = 2 * kEpiWarps;   // drain warps of both CTAs
 
@@ -111,61 +109,6 @@ struct DenseSmem {
     int failed;
 };
 
-__device__ __forceinline__ uint32_t saddr(const void* p) {
-    return static_cast<uint32_t>(__cvta_generic_to_shared(p));
-}
-__device__ __forceinline__ void mbar_init(unsigned long long* b, uint32_t count) {
-    asm volatile("mbarrier.init.shared::cta.b64 [%0], %1;" ::"r"(saddr(b)), "r"(count) : "memory");
-}
-__device__ __forceinline__ void mbar_expect_tx(unsigned long long* b, uint32_t bytes) {
-    asm volatile("{\n\t.reg .b64 st;\n\tmbarrier.arrive.expect_tx.shared::cta.b64 st, [%0], %1;\n\t}" ::"r"(saddr(b)),
-                 "r"(bytes)
-                 : "memory");
-}
-__device__ __forceinline__ bool mbar_test(unsigned long long* b, uint32_t parity) {
-    uint32_t ok;
-    asm volatile(
-        "{\n\t.reg .pred p;\n\tmbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2;\n\tselp.u32 %0, 1, 0, p;\n\t}"
-        : "=r"(ok)
-        : "r"(saddr(b)), "r"(parity)
-        : "memory");
-    return ok != 0;
-}
-// Arrive on the barrier at the same shared-memory offset in CTA `rank` of
-// this cluster (default semantics: release at CTA scope).  What the arrival
-// publishes is either tensor-core input in this CTA's shared memory, made
-// visible to the async proxy by fence.proxy.async beforehand, or the end of
-// this CTA's TMEM reads, ordered by tcgen05.fence::before_thread_sync.
-// (A release at cluster scope measured 750-1200 cycles per arrival here.)
-__device__ __forceinline__ void mbar_arrive_rank(unsigned long long* b, uint32_t rank) {
-    uint32_t remote;
-    asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(remote) : "r"(saddr(b)), "r"(rank));
-    asm volatile("mbarrier.arrive.shared::cluster.b64 _, [%0];" ::"r"(remote) : "memory");
-}
-__device__ __forceinline__ uint32_t cluster_rank() {
-    uint32_t r;
-    asm volatile("mov.u32 %0, %%cluster_ctarank;" : "=r"(r));
-    return r;
-}
-// Both CTAs of the pair reach this point (every thread of both).
-__device__ __forceinline__ void cluster_sync() {
-    asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
-}
-// Bounded wait: false when the clock limit ran out (which sets *failed) or, with
-// `failed` given, as soon as another role has failed.  Teardown waits pass
-// failed == nullptr and only give up on the limit.
-__device__ __forceinline__ bool mbar_wait(unsigned long long* b, uint32_t parity, volatile int* failed) {
-    const long long t0 = clock64();
-    while (!mbar_test(b, parity)) {
-        if (failed != nullptr && *failed) return false;
-        if (clock64() - t0 > kWaitCycles) {
-            if (failed != nullptr) *failed = 1;
-            return false;
-        }
-    }
-    return true;
-}
-
 __device__ __forceinline__ void tma_load_3d(void* dst, const CUtensorMap* map, int x, int y, int z,
                                             unsigned long long* bar) {
     asm volatile(
@@ -174,10 +117,6 @@ __device__ __forceinline__ void tma_load_3d(void* dst, const CUtensorMap* map, i
         "l"(map), "r"(x), "r"(y), "r"(z), "r"(saddr(bar))
         : "memory");
 }
-
-__device__ __forceinline__ void fence_proxy_async() { asm volatile("fence.proxy.async.shared::cta;" ::: "memory"); }
-__device__ __forceinline__ void tc_fence_before() { asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory"); }
-__device__ __forceinline__ void tc_fence_after() { asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory"); }
 
 // Shared-memory matrix descriptor (tcgen05 "version 1").
 // K-major: one row of kBK fp32 per M/N element -- the 64-byte swizzle
@@ -191,16 +130,6 @@ constexpr uint32_t kLayoutSW128Base32B = 1;
 constexpr uint32_t kLayoutKMajor = kBK == 32 ? 2u : 4u;
 constexpr uint32_t kSboKMajor = 8 * kBK * 4;
 static_assert(kBK == 16 || kBK == 32, "K block: one 64- or 128-byte swizzle row");
-__device__ __forceinline__ uint64_t smem_desc(uint32_t addr, uint32_t lbo, uint32_t sbo, uint32_t layout) {
-    uint64_t d = 0;
-    d |= uint64_t((addr >> 4) & 0x3FFF);
-    d |= uint64_t((lbo >> 4) & 0x3FFF) << 16;
-    d |= uint64_t((sbo >> 4) & 0x3FFF) << 32;
-    d |= uint64_t(1) << 46;  // descriptor version for sm_100
-    d |= uint64_t(layout & 7) << 61;
-    return d;
-}
-
 // Instruction descriptor of kind::tf32: D f32, A/B tf32, majors, N/8, M/16.
 __host__ __device__ constexpr uint32_t instr_desc(int M, int N, bool a_mn_major, bool b_mn_major) {
     return (1u << 4)                               // D format: f32
@@ -230,33 +159,6 @@ __device__ __forceinline__ void umma_commit_pair(unsigned long long* bar) {
             saddr(bar)),
         "h"(uint16_t(3))
         : "memory");
-}
-
-// 16 consecutive 32-bit columns of this warp's 32 TMEM lanes; the values
-// are valid after tmem_wait_ld.
-__device__ __forceinline__ void tmem_ld16(uint32_t taddr, uint32_t (&r)[16]) {
-    asm volatile(
-        "tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15}, [%16];"
-        : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]),
-          "=r"(r[8]), "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15])
-        : "r"(taddr));
-}
-// Waits for this thread's outstanding TMEM loads.  The registers pass through
-// the statement so that no use of them is scheduled ahead of the wait.
-__device__ __forceinline__ void tmem_wait_ld(uint32_t (&r)[16]) {
-    asm volatile("tcgen05.wait::ld.sync.aligned;"
-                 : "+r"(r[0]), "+r"(r[1]), "+r"(r[2]), "+r"(r[3]), "+r"(r[4]), "+r"(r[5]), "+r"(r[6]), "+r"(r[7]),
-                   "+r"(r[8]), "+r"(r[9]), "+r"(r[10]), "+r"(r[11]), "+r"(r[12]), "+r"(r[13]), "+r"(r[14]),
-                   "+r"(r[15])
-                 :
-                 : "memory");
-}
-// Orders later uses of r after the preceding volatile statement (a wait).
-__device__ __forceinline__ void reg_after(uint32_t (&r)[16]) {
-    asm volatile(""
-                 : "+r"(r[0]), "+r"(r[1]), "+r"(r[2]), "+r"(r[3]), "+r"(r[4]), "+r"(r[5]), "+r"(r[6]), "+r"(r[7]),
-                   "+r"(r[8]), "+r"(r[9]), "+r"(r[10]), "+r"(r[11]), "+r"(r[12]), "+r"(r[13]), "+r"(r[14]),
-                   "+r"(r[15]));
 }
 
 __device__ __forceinline__ float tf32_rn(float a) {
@@ -577,8 +479,26 @@ __global__ void dense_reduce_kernel(const float* __restrict__ P, int64_t nsplit,
     }
 }
 
-// ---- tensor maps (driver entry point fetched through the runtime) ----------
-PFN_cuTensorMapEncodeTiled_v12000 encode_fn() {
+// ---- tensor maps ------------------------------------------------------------
+// 3-D fp32 map: dims (innermost first), byte strides of dims 1 and 2, box.
+// K-major tiles use the 64- or 128-byte swizzle (one row per kBK floats),
+// MN-major tiles the 128-byte swizzle of 32-byte chunks (matching the
+// descriptors above).
+bool make_map(CUtensorMap* map, const void* base, const uint64_t dims[3], const uint64_t strides[2],
+              const uint32_t box[3], bool mn_major) {
+    auto fn = tensor_map_encoder();
+    if (fn == nullptr) return false;
+    const cuuint32_t elem_strides[3] = {1, 1, 1};
+    return fn(map, CU_TENSOR_MAP_DATA_TYPE_FLOAT32, 3, const_cast<void*>(base), dims, strides, box, elem_strides,
+              CU_TENSOR_MAP_INTERLEAVE_NONE,
+              mn_major ? CU_TENSOR_MAP_SWIZZLE_128B_ATOM_32B
+                       : (kBK == 32 ? CU_TENSOR_MAP_SWIZZLE_128B : CU_TENSOR_MAP_SWIZZLE_64B),
+              CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
+
+}  // namespace
+
+PFN_cuTensorMapEncodeTiled_v12000 tensor_map_encoder() {
     static PFN_cuTensorMapEncodeTiled_v12000 fn = nullptr;
     static std::once_flag once;
     std::call_once(once, [] {
@@ -591,28 +511,10 @@ PFN_cuTensorMapEncodeTiled_v12000 encode_fn() {
     return fn;
 }
 
-// 3-D fp32 map: dims (innermost first), byte strides of dims 1 and 2, box.
-// K-major tiles use the 64- or 128-byte swizzle (one row per kBK floats),
-// MN-major tiles the 128-byte swizzle of 32-byte chunks (matching the
-// descriptors above).
-bool make_map(CUtensorMap* map, const void* base, const uint64_t dims[3], const uint64_t strides[2],
-              const uint32_t box[3], bool mn_major) {
-    auto fn = encode_fn();
-    if (fn == nullptr) return false;
-    const cuuint32_t elem_strides[3] = {1, 1, 1};
-    return fn(map, CU_TENSOR_MAP_DATA_TYPE_FLOAT32, 3, const_cast<void*>(base), dims, strides, box, elem_strides,
-              CU_TENSOR_MAP_INTERLEAVE_NONE,
-              mn_major ? CU_TENSOR_MAP_SWIZZLE_128B_ATOM_32B
-                       : (kBK == 32 ? CU_TENSOR_MAP_SWIZZLE_128B : CU_TENSOR_MAP_SWIZZLE_64B),
-              CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
-}
-
-}  // namespace
-
 bool dense_f32_supported(int64_t nf, int64_t nt, int64_t ntasks, int64_t nobs, const void* X, const void* M) {
     return nf >= 32 && nf % 4 == 0 && nt >= 1 && ntasks >= 1 && nobs >= 1 && ntasks <= 65535 &&
            (reinterpret_cast<uintptr_t>(X) & 15u) == 0 && (reinterpret_cast<uintptr_t>(M) & 15u) == 0 &&
-           encode_fn() != nullptr;
+           tensor_map_encoder() != nullptr;
 }
 
 DensePlan dense_f32_plan(int64_t nf, int64_t nt, int64_t ntasks, int64_t nobs) {

@@ -2,8 +2,10 @@
 //
 // Per task, with X the matrix over its Frobenius norm and m <= n its sides:
 //   X <- (aI + bA + cA^2) X,  A = X X^T,
-// an odd polynomial of X's singular values.  Three products a step:
-//   A = X X^T,  B = aI + bA + cA A,  X' = B X.
+// an odd polynomial of X's singular values.  Short matrices (m <= 32) run in
+// double in one launch (glm_ortho_small.cu); the others take the norm and the
+// split of X into binary16 planes here, then three tensor-core products a step
+// (glm_ortho_gemm.cu).
 #include <algorithm>
 #include <cmath>
 
@@ -14,112 +16,111 @@ namespace glmb {
 namespace {
 
 constexpr int kThreads = 256;
-constexpr int kNormBlocks = 64;  // partial sums of a task's squared norm
-
-__device__ __forceinline__ double block_sum(double v, double* red) {
-#pragma unroll
-    for (int off = 16; off > 0; off >>= 1) v += __shfl_xor_sync(0xffffffffu, v, off);
-    if ((threadIdx.x & 31) == 0) red[threadIdx.x >> 5] = v;
-    __syncthreads();
-    double s = 0.0;
-    for (int w = 0; w < int(blockDim.x >> 5); ++w) s += red[w];
-    __syncthreads();
-    return s;
-}
-
-// The matrix to orthogonalise at element e: G itself, or the momentum's direction.
-template <typename T>
-__device__ __forceinline__ float direction(const T* G, const float* V, int64_t e, const OrthoUpdate& up) {
-    const float g = to_arith<float>(G[e]);
-    if (V == nullptr) return g;
-    return up.nesterov ? fmaf(up.mu, V[e], g) : V[e];
-}
 
 // part[task][block] = the block's share of |U|^2 in double; with a momentum, V <- mu V + G first.
+// One read of G (and a read and a write of V): bound by HBM.
 template <typename T>
 __global__ void __launch_bounds__(kThreads)
-    ortho_norm_kernel(const T* __restrict__ G, float* __restrict__ V, double* __restrict__ part, int64_t size,
-                      OrthoUpdate up) {
+    ortho_norm_kernel(const T* __restrict__ G, float* __restrict__ V, double* __restrict__ part,
+                      int* __restrict__ status, int64_t size, OrthoUpdate up) {
     __shared__ double red[kThreads / 32];
+    pdl_allow_dependents();
+    if (blockIdx.x == 0 && blockIdx.y == 0 && threadIdx.x == 0) *status = 0;
     const int64_t base = int64_t(blockIdx.y) * size;
+    const int64_t stride = int64_t(gridDim.x) * kThreads;
     double s = 0.0;
-    for (int64_t i = int64_t(blockIdx.x) * kThreads + threadIdx.x; i < size; i += int64_t(gridDim.x) * kThreads) {
-        if (V != nullptr) V[base + i] = fmaf(up.mu, V[base + i], to_arith<float>(G[base + i]));
-        const double u = double(direction(G, V, base + i, up));
-        s += u * u;
+    int64_t i = int64_t(blockIdx.x) * kThreads + threadIdx.x;
+    auto one = [&](float g, float v, int64_t e) {
+        float u = g;
+        if (V != nullptr) {
+            v = fmaf(up.mu, v, g);
+            V[e] = v;
+            u = up.nesterov ? fmaf(up.mu, v, g) : v;
+        }
+        s = fma(double(u), double(u), s);
+    };
+    constexpr int kAhead = 8;
+    for (; i + (kAhead - 1) * stride < size; i += kAhead * stride) {
+        float g[kAhead], v[kAhead];
+#pragma unroll
+        for (int j = 0; j < kAhead; ++j) {
+            g[j] = to_arith<float>(G[base + i + j * stride]);
+            v[j] = V != nullptr ? V[base + i + j * stride] : 0.0f;
+        }
+#pragma unroll
+        for (int j = 0; j < kAhead; ++j) one(g[j], v[j], base + i + j * stride);
     }
-    s = block_sum(s, red);
-    if (threadIdx.x == 0) part[int64_t(blockIdx.y) * gridDim.x + blockIdx.x] = s;
+    for (; i < size; i += stride)
+        one(to_arith<float>(G[base + i]), V != nullptr ? V[base + i] : 0.0f, base + i);
+#pragma unroll
+    for (int off = 16; off > 0; off >>= 1) s += __shfl_xor_sync(0xffffffffu, s, off);
+    if ((threadIdx.x & 31) == 0) red[threadIdx.x >> 5] = s;
+    __syncthreads();
+    if (threadIdx.x == 0) {
+        double t = 0.0;
+        for (int w = 0; w < kThreads / 32; ++w) t += red[w];
+        part[int64_t(blockIdx.y) * gridDim.x + blockIdx.x] = t;
+    }
 }
 
-// X[task][i][j] = U / |U|, transposed when the matrix is taller than wide.
+// 64 x 64 tiles of X = scale * U / |U| into its planes, transposed when the matrix is taller than wide;
+// columns that fill up a row to ld (and rows past m: none) are zero.
 template <typename T>
 __global__ void __launch_bounds__(kThreads)
-    ortho_init_kernel(const T* __restrict__ G, const float* __restrict__ V, const double* __restrict__ part,
-                      float* __restrict__ X, int64_t m, int64_t n, bool tall, OrthoUpdate up) {
-    double ss = 0.0;
-    for (int i = 0; i < kNormBlocks; ++i) ss += part[int64_t(blockIdx.y) * kNormBlocks + i];
-    const double inv = ss == 0.0 ? 0.0 : 1.0 / sqrt(ss);
-    const int64_t size = m * n, base = int64_t(blockIdx.y) * size;
-    for (int64_t e = int64_t(blockIdx.x) * kThreads + threadIdx.x; e < size; e += int64_t(gridDim.x) * kThreads) {
-        const int64_t i = e / n, j = e % n;
-        X[base + e] = float(double(direction(G, V, base + (tall ? j * m + i : e), up)) * inv);
+    ortho_split_kernel(const T* __restrict__ G, const float* __restrict__ V, const double* __restrict__ part, int nparts,
+                       __half* __restrict__ X, int64_t m, int64_t n, int64_t ld, bool tall, float scale, OrthoUpdate up) {
+    __shared__ float t[64][65];
+    __shared__ double inv_s;
+    pdl_allow_dependents();
+    pdl_wait_for_producer();
+    const int64_t task = blockIdx.z, base = task * m * n;
+    if (threadIdx.x < 32) {
+        double ss = 0.0;
+        for (int i = threadIdx.x; i < nparts; i += 32) ss += part[task * nparts + i];
+#pragma unroll
+        for (int off = 16; off > 0; off >>= 1) ss += __shfl_xor_sync(0xffffffffu, ss, off);
+        if (threadIdx.x == 0) inv_s = ss == 0.0 ? 0.0 : double(scale) / sqrt(ss);
+    }
+    const int64_t tiles_n = (n + 63) / 64, tiles = tiles_n * ((m + 63) / 64);
+    __syncthreads();
+    const double inv = inv_s;
+    for (int64_t tile = blockIdx.x; tile < tiles; tile += gridDim.x) {
+        const int64_t i0 = tile / tiles_n * 64, j0 = tile % tiles_n * 64;
+#pragma unroll 4
+        for (int e = threadIdx.x; e < 64 * 64; e += kThreads) {
+            // neighbouring threads on neighbouring elements of the matrix as it lies in memory
+            const int i = tall ? e & 63 : e >> 6, j = tall ? e >> 6 : e & 63;
+            float v = 0.0f;
+            if (i0 + i < m && j0 + j < n) {
+                const int64_t at = base + (tall ? (j0 + j) * m + i0 + i : (i0 + i) * n + j0 + j);
+                v = float(double(ortho_direction(G, V, at, up)) * inv);
+            }
+            t[i][j] = v;
+        }
+        __syncthreads();
+#pragma unroll 4
+        for (int e = threadIdx.x; e < 64 * 32; e += kThreads) {
+            const int i = e >> 5, j = 2 * (e & 31);
+            if (i0 + i < m && j0 + j < ld) {
+                const float a = t[i][j], b = t[i][j + 1];
+                const __half2 h = __floats2half2_rn(a, b);
+                const float2 f = __half22float2(h);
+                __half* dst = X + (task * 2 * m + i0 + i) * ld + j0 + j;
+                *reinterpret_cast<__half2*>(dst) = h;
+                *reinterpret_cast<__half2*>(dst + m * ld) = __floats2half2_rn(a - f.x, b - f.y);
+            }
+        }
+        __syncthreads();
     }
 }
 
-// D[rows x cols] = alpha * P Q (+ beta * C) (+ gamma on the diagonal), Q read as Q[c][k] when QT.
-template <bool QT>
-__global__ void __launch_bounds__(256)
-    ortho_gemm_kernel(const float* __restrict__ P, const float* __restrict__ Q, const float* C, float* __restrict__ D,
-                      int64_t rows, int64_t cols, int64_t K, int64_t p_task, int64_t q_task, int64_t d_task,
-                      float alpha, float beta, float gamma) {
-    __shared__ float sp[16][68], sq[16][68];
-    const int64_t task = blockIdx.z, r0 = int64_t(blockIdx.y) * 64, c0 = int64_t(blockIdx.x) * 64;
-    P += task * p_task;
-    Q += task * q_task;
-    const int tx = threadIdx.x & 15, ty = threadIdx.x >> 4;
-    float acc[4][4] = {};
-    for (int64_t k0 = 0; k0 < K; k0 += 16) {
-        for (int i = threadIdx.x; i < 1024; i += 256) {
-            const int r = i >> 4, k = i & 15;
-            sp[k][r] = r0 + r < rows && k0 + k < K ? P[(r0 + r) * K + k0 + k] : 0.0f;
-            if (QT) sq[k][r] = c0 + r < cols && k0 + k < K ? Q[(c0 + r) * K + k0 + k] : 0.0f;
-            const int c = i & 63, kk = i >> 6;
-            if (!QT) sq[kk][c] = c0 + c < cols && k0 + kk < K ? Q[(k0 + kk) * cols + c0 + c] : 0.0f;
-        }
-        __syncthreads();
-#pragma unroll
-        for (int k = 0; k < 16; ++k)
-#pragma unroll
-            for (int i = 0; i < 4; ++i)
-#pragma unroll
-                for (int j = 0; j < 4; ++j) acc[i][j] = fmaf(sp[k][ty * 4 + i], sq[k][tx * 4 + j], acc[i][j]);
-        __syncthreads();
-    }
-    for (int i = 0; i < 4; ++i)
-        for (int j = 0; j < 4; ++j) {
-            const int64_t r = r0 + ty * 4 + i, c = c0 + tx * 4 + j;
-            if (r >= rows || c >= cols) continue;
-            const int64_t e = task * d_task + r * cols + c;
-            float v = alpha * acc[i][j];
-            if (C != nullptr) v = fmaf(beta, C[e], v);
-            if (r == c) v += gamma;
-            D[e] = v;
-        }
+// Blocks a task's norm is shared by: enough for the memory system, 4096 elements each at the least.
+int64_t norm_blocks(int64_t size, int64_t ntasks) {
+    const int64_t most = std::max<int64_t>(1, 8 * int64_t(sm_count()) / std::max<int64_t>(1, ntasks));
+    return std::max<int64_t>(1, std::min(most, (size + 4095) / 4096));
 }
 
-template <typename T>
-__global__ void __launch_bounds__(kThreads)
-    ortho_store_kernel(const float* __restrict__ X, T* __restrict__ out, int64_t m, int64_t n, bool tall, bool update,
-                       OrthoUpdate up) {
-    const int64_t size = m * n, base = int64_t(blockIdx.y) * size;
-    for (int64_t e = int64_t(blockIdx.x) * kThreads + threadIdx.x; e < size; e += int64_t(gridDim.x) * kThreads) {
-        const int64_t o = base + (tall ? (e % n) * m + e / n : e);
-        float v = X[base + e];
-        if (update) v = fmaf(-up.rate, v, up.keep * to_arith<float>(out[o]));
-        out[o] = from_arith<T>(v);
-    }
-}
+int64_t padded(int64_t cols) { return (cols + 7) / 8 * 8; }
 
 }  // namespace
 
@@ -162,8 +163,9 @@ int ortho_plan_steps(const double* coefficients, int steps, OrthoSteps* out) {
 template <typename T>
 size_t ortho_workspace(int64_t nf, int64_t nt, int64_t ntasks) {
     const int64_t m = std::min(nf, nt), n = std::max(nf, nt);
-    return round_up(size_t(ntasks) * kNormBlocks * 8, 256) +
-           2 * round_up(size_t(ntasks) * m * n * 4, 256) + 2 * round_up(size_t(ntasks) * m * m * 4, 256);
+    if (m <= kOrthoSmallRows) return 0;
+    return 256 + round_up(size_t(ntasks) * norm_blocks(m * n, ntasks) * 8, 256) +
+           2 * round_up(size_t(ntasks) * m * padded(n) * 4, 256) + 2 * round_up(size_t(ntasks) * m * padded(m) * 4, 256);
 }
 
 template <typename T>
@@ -171,39 +173,41 @@ int ortho_run(const T* G, float* V, T* out, int64_t nf, int64_t nt, int64_t ntas
               const OrthoUpdate* update, void* ws, size_t ws_bytes, cudaStream_t stream) {
     const int64_t m = std::min(nf, nt), n = std::max(nf, nt), size = m * n;
     const bool tall = nt > nf;
-    if (ntasks > 65535) return GLMB_ERR_TOO_LARGE;
+    if (m <= kOrthoSmallRows) {
+        set_last_path("ortho_small");
+        return ortho_small<T>(G, V, out, m, n, tall, ntasks, steps, update, stream);
+    }
+    if (ntasks > 65535 || n > (int64_t(1) << 30)) return GLMB_ERR_TOO_LARGE;
     Scratch sc(ws, ws_bytes, ortho_workspace<T>(nf, nt, ntasks), stream);
     if (sc.status() != GLMB_OK) return sc.status();
-    char* w = sc.as<char>();
+    char* w = sc.template as<char>();
     auto take = [&](size_t bytes) {
         char* p = w;
         w += round_up(bytes, 256);
         return p;
     };
-    double* part = reinterpret_cast<double*>(take(size_t(ntasks) * kNormBlocks * 8));
-    float* X = reinterpret_cast<float*>(take(size_t(ntasks) * size * 4));
-    float* X2 = reinterpret_cast<float*>(take(size_t(ntasks) * size * 4));
-    float* A = reinterpret_cast<float*>(take(size_t(ntasks) * m * m * 4));
-    float* B = reinterpret_cast<float*>(take(size_t(ntasks) * m * m * 4));
+    OrthoPlanes p{m, n, padded(m), padded(n), ntasks, {}, nullptr, nullptr};
+    int* status = reinterpret_cast<int*>(take(4));
+    const int64_t nb = norm_blocks(size, ntasks);
+    double* part = reinterpret_cast<double*>(take(size_t(ntasks) * nb * 8));
+    for (__half*& x : p.X) x = reinterpret_cast<__half*>(take(size_t(ntasks) * m * p.ld_n * 4));
+    p.A = reinterpret_cast<__half*>(take(size_t(ntasks) * m * p.ld_m * 4));
+    p.B = reinterpret_cast<__half*>(take(size_t(ntasks) * m * p.ld_m * 4));
     const OrthoUpdate up = update != nullptr ? *update : OrthoUpdate{};
-    const unsigned eb = unsigned(std::min<int64_t>(1024, (size + kThreads - 1) / kThreads));
-    set_last_path("ortho");
-    ortho_norm_kernel<T><<<dim3(kNormBlocks, unsigned(ntasks)), kThreads, 0, stream>>>(G, V, part, size, up);
-    ortho_init_kernel<T><<<dim3(eb, unsigned(ntasks)), kThreads, 0, stream>>>(G, V, part, X, m, n, tall, up);
-    const unsigned mt = unsigned((m + 63) / 64), ntl = unsigned((n + 63) / 64);
-    for (int k = 0; k < steps.n; ++k) {
-        const OrthoStep& s = steps.step[k];
-        ortho_gemm_kernel<true><<<dim3(mt, mt, unsigned(ntasks)), 256, 0, stream>>>(X, X, nullptr, A, m, m, n, size, size,
-                                                                                    m * m, 1.0f, 0.0f, 0.0f);
-        ortho_gemm_kernel<true><<<dim3(mt, mt, unsigned(ntasks)), 256, 0, stream>>>(A, A, A, B, m, m, m, m * m, m * m,
-                                                                                    m * m, s.c, s.b, s.a);
-        ortho_gemm_kernel<false><<<dim3(ntl, mt, unsigned(ntasks)), 256, 0, stream>>>(B, X, nullptr, X2, m, n, m, m * m,
-                                                                                      size, size, 1.0f, 0.0f, 0.0f);
-        std::swap(X, X2);
-    }
-    ortho_store_kernel<T><<<dim3(eb, unsigned(ntasks)), kThreads, 0, stream>>>(X, out, m, n, tall, update != nullptr, up);
-    count_launch(3 + 3 * steps.n);
-    return launch_status();
+    set_last_path("ortho_tensor");
+    ortho_norm_kernel<T><<<dim3(unsigned(nb), unsigned(ntasks)), kThreads, 0, stream>>>(G, V, part, status, size, up);
+    count_launch();
+    int st = launch_status();
+    if (st != GLMB_OK) return st;
+    const int64_t tiles = (n + 63) / 64 * ((m + 63) / 64);
+    const int64_t most = std::max<int64_t>(1, 8 * int64_t(sm_count()) / ntasks);
+    const cudaError_t e =
+        pdl_launch(ortho_split_kernel<T>, dim3(unsigned(std::min(tiles, most)), 1, unsigned(ntasks)), dim3(kThreads), 0,
+                   stream, G, static_cast<const float*>(V), static_cast<const double*>(part), int(nb), p.X[0], m, n,
+                   p.ld_n, tall, ortho_x_scale(steps.step[0]), up);
+    count_launch();
+    if (e != cudaSuccess) return int(e);
+    return ortho_products<T>(p, steps, out, tall, update, status, stream);
 }
 
 #define GLMB_INSTANTIATE_ORTHO(T)                                                                                \

@@ -29,6 +29,35 @@ struct OrthoUpdate {
     float keep, rate;
 };
 
+// What orthogonalises when m (the shorter side) is large: binary16 planes [task][2: hi, lo][rows][ld].
+struct OrthoPlanes {
+    int64_t m, n, ld_m, ld_n, ntasks;
+    __half* X[2];  // m x n, before and after a step in turn
+    __half* A;     // m x m
+    __half* B;
+};
+// The power of two that X's planes carry before a step.
+float ortho_x_scale(const OrthoStep& s);
+// All steps from X[0] (scaled by ortho_x_scale of the first) to `out` or, with `up`, the model's update;
+// *status != 0 makes the outputs NaN (glm_ortho_gemm.cu).
+template <typename T>
+int ortho_products(const OrthoPlanes& p, const OrthoSteps& steps, T* out, bool tall, const OrthoUpdate* up, int* status,
+                   cudaStream_t stream);
+
+// m <= kOrthoSmallRows: one launch in double (glm_ortho_small.cu).
+constexpr int64_t kOrthoSmallRows = 32;
+template <typename T>
+int ortho_small(const T* G, float* V, T* out, int64_t m, int64_t n, bool tall, int64_t ntasks, const OrthoSteps& steps,
+                const OrthoUpdate* up, cudaStream_t stream);
+
+// The matrix to orthogonalise at element e: G itself, or the (updated) momentum's direction.
+template <typename T>
+__device__ __forceinline__ float ortho_direction(const T* G, const float* V, int64_t e, const OrthoUpdate& up) {
+    const float g = to_arith<float>(G[e]);
+    if (V == nullptr) return g;
+    return up.nesterov ? fmaf(up.mu, V[e], g) : V[e];
+}
+
 template <typename T>
 size_t ortho_workspace(int64_t nf, int64_t nt, int64_t ntasks);
 // out = O(G); with `up`, G is the gradient, V the momentum and out the model.  out may be G (up == nullptr).

@@ -1,0 +1,627 @@
+// glm_ortho_gemm.cu -- the three products of a Newton-Schulz step on the
+// 5th-generation tensor cores:
+//   A = X X^T,   B = aI + bA + cA A,   X' = B X      (X: m x n, m <= n).
+//
+// Operands are pairs of binary16 values, hi = the value rounded to nearest and
+// lo = the rest rounded to nearest, after a scaling by a power of two that the
+// host derives from the bound on X's singular values (glm_ortho.cuh): 22
+// significant bits, and an absolute 2^-25 of the scaled unit at the least.  A
+// product takes three MMAs (hi*lo + lo*hi + hi*hi; the dropped lo*lo is 2^-22
+// of the product), at twice the rate of tf32 and half its bytes.  Normalised
+// iterates make this possible: nothing in X, A or B can leave binary16's range.
+//
+// The tensor core cuts towards zero where it accumulates, so each 64-deep
+// block of K is accumulated from zero in one of two TMEM buffers (small
+// corrections first) and eight warps add it into float registers, rounding to
+// nearest, while the tensor core fills the other buffer.
+//
+// A and B are symmetric: only the tiles on and above the diagonal are
+// computed, and the epilogue writes each tile and its mirror image.
+//
+// Two tile shapes.  PAIR: 256 x 256 on a CTA pair (cta_group::2), each CTA
+// staging its 128 rows of the left operand and 128 of the 256 columns of the
+// right one -- 64 KB for 1536 clocks of MMA, where a 128 x 128 tile of one CTA
+// brings in the same bytes for half the work.  Single: 128 x 128 on one CTA,
+// for products with too few large tiles.  Either may split K over the CTAs
+// (pairs) of a cluster: every CTA leaves its partial tile in its shared
+// memory and sums its share of the rows over its peers', in rank order.
+#include <algorithm>
+#include <cmath>
+
+#include "glm_ortho.cuh"
+#include "glm_tc.cuh"
+
+namespace glmb {
+
+namespace {
+
+constexpr int kBM = 128;  // rows of D per CTA
+constexpr int kBK = 64;   // K per stage: 128 bytes of binary16, one swizzle row
+constexpr int kStages = 3;
+constexpr int kPlaneBytes = 128 * kBK * 2;  // 128 rows (or columns) of one plane: 16 KB
+constexpr int kStageBytes = 4 * kPlaneBytes;  // left hi, lo, right hi, lo
+constexpr int kDrainWarp0 = 4, kDrainWarps = 8, kDrainThreads = kDrainWarps * 32;
+constexpr int kThreads = (kDrainWarp0 + kDrainWarps) * 32;
+// 384 threads launch with 168 registers each; the control warpgroup gives its share to the two that drain
+constexpr uint32_t kRegsControl = 72, kRegsDrain = 208;
+static_assert(128 * kRegsControl + 256 * kRegsDrain <= kThreads * 168, "register split exceeds the launch");
+
+struct GemmSmem {
+    alignas(1024) unsigned char stage[kStages][kStageBytes];  // later the float tile
+    unsigned long long full[kStages];
+    unsigned long long ready[kStages];  // (even CTA of a pair) the odd CTA's copies have landed
+    unsigned long long empty[kStages];
+    unsigned long long accf[2];
+    unsigned long long acce[2];
+    unsigned long long done;
+    uint32_t tmem_base;
+    int failed;
+};
+
+// D (f32) from binary16 A and B; K-major A, B K- or MN-major.
+constexpr uint32_t instr_desc_f16(int M, int N, bool b_mn_major) {
+    return (1u << 4) | (uint32_t(b_mn_major) << 16) | (uint32_t(N >> 3) << 17) | (uint32_t(M >> 4) << 24);
+}
+
+constexpr uint32_t kLayoutSW128 = 2;
+
+template <bool PAIR>
+__device__ __forceinline__ void mma_f16(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t accumulate) {
+    if constexpr (PAIR)
+        asm volatile(
+            "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\t"
+            "tcgen05.mma.cta_group::2.kind::f16 [%0], %1, %2, %3, p;\n\t}" ::"r"(d),
+            "l"(a), "l"(b), "r"(idesc), "r"(accumulate)
+            : "memory");
+    else
+        asm volatile(
+            "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\t"
+            "tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}" ::"r"(d),
+            "l"(a), "l"(b), "r"(idesc), "r"(accumulate)
+            : "memory");
+}
+
+// One arrival on `bar` (in both CTAs of a pair, `mask` their cluster ranks) once the MMAs issued so far retire.
+template <bool PAIR>
+__device__ __forceinline__ void commit(unsigned long long* bar, uint16_t mask) {
+    if constexpr (PAIR)
+        asm volatile(
+            "tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64 [%0], %1;" ::"r"(
+                saddr(bar)),
+            "h"(mask)
+            : "memory");
+    else
+        asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(saddr(bar))
+                     : "memory");
+}
+
+__device__ __forceinline__ void tma_load_4d(void* dst, const CUtensorMap* map, int x, int y, int z, int w,
+                                            unsigned long long* bar) {
+    asm volatile(
+        "cp.async.bulk.tensor.4d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4, %5}], [%6];" ::
+            "r"(saddr(dst)),
+        "l"(map), "r"(x), "r"(y), "r"(z), "r"(w), "r"(saddr(bar))
+        : "memory");
+}
+
+__device__ __forceinline__ float4 ld_cluster_f4(uint32_t addr) {
+    float4 v;
+    asm volatile("ld.shared::cluster.v4.f32 {%0,%1,%2,%3}, [%4];"
+                 : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w)
+                 : "r"(addr)
+                 : "memory");
+    return v;
+}
+__device__ __forceinline__ int ld_cluster_s32(uint32_t addr) {
+    int v;
+    asm volatile("ld.shared::cluster.s32 %0, [%1];" : "=r"(v) : "r"(addr) : "memory");
+    return v;
+}
+__device__ __forceinline__ uint32_t mapa(uint32_t addr, uint32_t rank) {
+    uint32_t r;
+    asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(r) : "r"(addr), "r"(rank));
+    return r;
+}
+__device__ __forceinline__ void drain_sync() { asm volatile("bar.sync 1, %0;" ::"n"(kDrainThreads) : "memory"); }
+
+__device__ __forceinline__ uint32_t pack_half2(float a, float b) {
+    const __half2 h = __floats2half2_rn(a, b);
+    return *reinterpret_cast<const uint32_t*>(&h);
+}
+// v ~ hi + lo of two values
+__device__ __forceinline__ void split_half2(float a, float b, uint32_t& hi, uint32_t& lo) {
+    const __half2 h = __floats2half2_rn(a, b);
+    const float2 f = __half22float2(h);
+    hi = *reinterpret_cast<const uint32_t*>(&h);
+    lo = pack_half2(a - f.x, b - f.y);
+}
+
+enum : int { kGram, kPoly, kApply, kLast };
+
+struct GemmArgs {
+    int64_t m, n;       // rows and columns of D
+    int32_t tiles_m, tiles_n;  // tiles of D (kGram, kPoly: tiles_m of them on a side)
+    int32_t units;      // tiles a task has
+    int32_t nkb;        // 64-deep blocks of K
+    int32_t splits;     // CTAs (pairs) of a cluster, each with its share of K
+    float scale;        // of the accumulated sum
+    float a, b;         // kPoly: on the diagonal, times A
+    const __half* A;    // kPoly: A's planes (D's layout)
+    __half* D;          // planes [task][2][m][ld]
+    int64_t ld;
+    void* out;          // kLast
+    bool tall, update;
+    float keep, rate;
+    int* status;
+};
+
+template <bool PAIR, int KIND, typename T>
+__global__ void __launch_bounds__(kThreads, 1)
+    ortho_gemm_kernel(const __grid_constant__ CUtensorMap map_left, const __grid_constant__ CUtensorMap map_right,
+                      const GemmArgs a) {
+    constexpr int kBN = PAIR ? 256 : 128;   // columns of a tile
+    constexpr int kBT = PAIR ? 256 : 128;   // rows of a tile (of both CTAs)
+    constexpr int kCols = kBN / 2;          // columns a drain thread sums
+    constexpr uint32_t kTmemCols = 2 * kBN;
+    constexpr int kTileLd = kBN + 4;        // floats; four banks on from row to row
+    static_assert(kBM * kTileLd * 4 <= kStages * kStageBytes);
+    constexpr bool kSym = KIND == kGram || KIND == kPoly;
+
+    extern __shared__ __align__(1024) unsigned char smem_raw[];
+    GemmSmem& sm = *reinterpret_cast<GemmSmem*>(
+        reinterpret_cast<unsigned char*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023)));
+    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+    const uint32_t rank = cluster_rank();
+    const uint32_t half = PAIR ? (rank & 1) : 0;          // which CTA of the pair
+    const uint32_t part = PAIR ? (rank >> 1) : rank;      // which share of K
+    const uint32_t lead = PAIR ? (rank & ~1u) : rank;     // the CTA that issues the MMAs
+    const int csize = a.splits * (PAIR ? 2 : 1);
+
+    const int64_t cluster = blockIdx.x / csize;
+    const int64_t task = cluster / a.units;
+    const int u = int(cluster % a.units);
+    int ti, tj;
+    if constexpr (kSym) {
+        // u counts the tiles (ti <= tj) column by column: u = tj (tj + 1) / 2 + ti
+        tj = int((sqrtf(8.0f * float(u) + 1.0f) - 1.0f) * 0.5f);
+        while (tj * (tj + 1) / 2 > u) --tj;
+        while ((tj + 1) * (tj + 2) / 2 <= u) ++tj;
+        ti = u - tj * (tj + 1) / 2;
+    } else {
+        // bands of eight tile rows, walked column by column: tiles that run together share both operands
+        const int band = u / (8 * a.tiles_n), first = band * 8, rows = min(8, a.tiles_m - first);
+        const int in = u - band * 8 * a.tiles_n;
+        ti = first + in % rows;
+        tj = in / rows;
+    }
+    const int m0 = ti * kBT + int(half) * kBM;       // this CTA's rows of D
+    const int n0 = tj * kBN;
+    const int nb0 = n0 + int(half) * 128;            // the columns this CTA stages
+    // this CTA's share of K
+    const int kb0 = int(int64_t(a.nkb) * part / a.splits), kb1 = int(int64_t(a.nkb) * (part + 1) / a.splits);
+    const int nkb = kb1 - kb0;
+
+    if (tid == 0) {
+        for (int s = 0; s < kStages; ++s) {
+            mbar_init(&sm.full[s], 1);
+            mbar_init(&sm.ready[s], 1);
+            mbar_init(&sm.empty[s], 1);
+        }
+        for (int b = 0; b < 2; ++b) {
+            mbar_init(&sm.accf[b], 1);
+            mbar_init(&sm.acce[b], (PAIR ? 2 : 1) * kDrainWarps);
+        }
+        mbar_init(&sm.done, 1);
+        sm.failed = 0;
+        asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+    }
+    if (warp == 1) {
+        if constexpr (PAIR) {
+            asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(saddr(&sm.tmem_base)),
+                         "r"(kTmemCols)
+                         : "memory");
+            asm volatile("tcgen05.relinquish_alloc_permit.cta_group::2.sync.aligned;" ::: "memory");
+        } else {
+            asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(saddr(&sm.tmem_base)),
+                         "r"(kTmemCols)
+                         : "memory");
+            asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+        }
+    }
+    tc_fence_before();
+    __syncthreads();
+    cluster_sync();  // the peers' barriers exist before anyone arrives on them
+    tc_fence_after();
+    const uint32_t tmem = sm.tmem_base;
+    volatile int* failed = &sm.failed;
+    float* tile = reinterpret_cast<float*>(sm.stage[0]);
+    pdl_allow_dependents();
+    pdl_wait_for_producer();
+
+    if (warp < kDrainWarp0) {
+        asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kRegsControl));
+        if (warp == 0 && lane == 0) {
+            int issued = 0;
+            for (int kb = 0; kb < nkb; ++kb) {
+                const int s = kb % kStages;
+                if (kb >= kStages && !mbar_wait(&sm.empty[s], uint32_t((kb / kStages - 1) & 1), failed)) break;
+                unsigned char* st = sm.stage[s];
+                const int k = (kb0 + kb) * kBK;
+                mbar_expect_tx(&sm.full[s], kStageBytes);
+                tma_load_4d(st, &map_left, k, m0, 0, int(task), &sm.full[s]);
+                if constexpr (kSym) {
+                    tma_load_4d(st + 2 * kPlaneBytes, &map_right, k, nb0, 0, int(task), &sm.full[s]);
+                } else {
+                    // two atoms of 64 columns x 64 rows of X, hi and lo each
+                    tma_load_4d(st + 2 * kPlaneBytes, &map_right, nb0, k, 0, int(task), &sm.full[s]);
+                    tma_load_4d(st + 3 * kPlaneBytes, &map_right, nb0 + 64, k, 0, int(task), &sm.full[s]);
+                }
+                issued = kb + 1;
+            }
+            // the copies still in flight land before shared memory is used for anything else
+            for (int kb = issued > kStages ? issued - kStages : 0; kb < issued; ++kb)
+                mbar_wait(&sm.full[kb % kStages], uint32_t((kb / kStages) & 1), nullptr);
+        } else if (warp == 1 && lane == 0) {
+            if (rank == lead) {
+                constexpr uint32_t idesc = instr_desc_f16(kBT, kBN, !kSym);
+                const uint16_t mask = uint16_t(PAIR ? 3u << lead : 0u);
+                for (int kb = 0; kb < nkb; ++kb) {
+                    const int s = kb % kStages, buf = kb & 1;
+                    if (kb >= 2 && !mbar_wait(&sm.acce[buf], uint32_t(((kb >> 1) - 1) & 1), failed)) break;
+                    if (!mbar_wait(&sm.full[s], uint32_t((kb / kStages) & 1), failed)) break;
+                    if (PAIR && !mbar_wait(&sm.ready[s], uint32_t((kb / kStages) & 1), failed)) break;
+                    tc_fence_after();
+                    const uint32_t base = saddr(sm.stage[s]);
+                    const uint32_t d = tmem + uint32_t(buf * kBN);
+                    uint64_t lh[kBK / 16], ll[kBK / 16], rh[kBK / 16], rl[kBK / 16];
+#pragma unroll
+                    for (int k = 0; k < kBK / 16; ++k) {
+                        // K-major: 16 binary16 = 32 bytes on along the row; 8-row groups 1024 bytes apart
+                        lh[k] = smem_desc(base + 32 * k, 16, 1024, kLayoutSW128);
+                        ll[k] = smem_desc(base + kPlaneBytes + 32 * k, 16, 1024, kLayoutSW128);
+                        if constexpr (kSym) {
+                            rh[k] = smem_desc(base + 2 * kPlaneBytes + 32 * k, 16, 1024, kLayoutSW128);
+                            rl[k] = smem_desc(base + 3 * kPlaneBytes + 32 * k, 16, 1024, kLayoutSW128);
+                        } else {
+                            // MN-major: 16 K-rows of 128 bytes on; 8-row groups 1024 bytes, 64-column atoms
+                            // (hi and lo of one, then of the next) a plane apart
+                            rh[k] = smem_desc(base + 2 * kPlaneBytes + 2048 * k, kPlaneBytes, 1024, kLayoutSW128);
+                            rl[k] = smem_desc(base + 2 * kPlaneBytes + kPlaneBytes / 2 + 2048 * k, kPlaneBytes, 1024,
+                                              kLayoutSW128);
+                        }
+                    }
+#pragma unroll
+                    for (int k = 0; k < kBK / 16; ++k) {
+                        mma_f16<PAIR>(d, ll[k], rh[k], idesc, k > 0 ? 1u : 0u);
+                        mma_f16<PAIR>(d, lh[k], rl[k], idesc, 1u);
+                    }
+#pragma unroll
+                    for (int k = 0; k < kBK / 16; ++k) mma_f16<PAIR>(d, lh[k], rh[k], idesc, 1u);
+                    commit<PAIR>(&sm.empty[s], mask);
+                    commit<PAIR>(&sm.accf[buf], mask);
+                }
+                commit<PAIR>(&sm.done, mask);
+            }
+            mbar_wait(&sm.done, 0, nullptr);
+        } else if (PAIR && warp == 2 && lane == 0 && rank != lead) {
+            // tells the even CTA that this CTA's copies of a stage have landed
+            for (int kb = 0; kb < nkb; ++kb) {
+                const int s = kb % kStages;
+                if (!mbar_wait(&sm.full[s], uint32_t((kb / kStages) & 1), failed)) break;
+                fence_proxy_async();
+                mbar_arrive_rank(&sm.ready[s], lead);
+            }
+        }
+    } else {
+        asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kRegsDrain));
+        const int quarter = warp & 3, side = (warp - kDrainWarp0) >> 2;
+        const uint32_t tbase = tmem + (uint32_t(32 * quarter) << 16) + uint32_t(side * kCols);
+        float sum[kCols];
+#pragma unroll
+        for (int i = 0; i < kCols; ++i) sum[i] = 0.0f;
+        bool ok = true;
+        for (int kb = 0; kb < nkb; ++kb) {
+            const int buf = kb & 1;
+            if (!(ok = mbar_wait(&sm.accf[buf], uint32_t((kb >> 1) & 1), failed))) break;
+            tc_fence_after();
+#pragma unroll
+            for (int h = 0; h < kCols / 32; ++h) {
+                uint32_t r[2][16];
+                tmem_ld16(tbase + uint32_t(buf * kBN + 32 * h), r[0]);
+                tmem_ld16(tbase + uint32_t(buf * kBN + 32 * h + 16), r[1]);
+                tmem_wait_ld(r[0]);
+                reg_after(r[1]);
+#pragma unroll
+                for (int j = 0; j < 2; ++j)
+#pragma unroll
+                    for (int i = 0; i < 16; ++i) sum[32 * h + 16 * j + i] += __uint_as_float(r[j][i]);
+            }
+            tc_fence_before();
+            __syncwarp();
+            if (lane == 0) mbar_arrive_rank(&sm.acce[buf], lead);
+        }
+        // every copy has landed and every MMA of this CTA's stages has retired: the stages become the tile
+        if (ok) {
+            float* row = tile + (32 * quarter + lane) * kTileLd + side * kCols;
+#pragma unroll
+            for (int i = 0; i < kCols; i += 4)
+                *reinterpret_cast<float4*>(row + i) = make_float4(sum[i], sum[i + 1], sum[i + 2], sum[i + 3]);
+        }
+    }
+    tc_fence_before();
+    __syncthreads();
+    if (csize > 1) cluster_sync();  // the peers' partial tiles are complete
+
+    if (warp >= kDrainWarp0) {
+        const int ew = warp - kDrainWarp0;
+        const int share = kBM / a.splits;  // rows of the tile this CTA finishes
+        const int r0 = int(part) * share;
+        const bool mirror = kSym && ti != tj;
+        bool bad = false;
+        if constexpr (KIND == kLast) {
+            bad = *static_cast<volatile int*>(a.status) != 0;
+            for (int p = 0; p < csize; ++p) bad |= ld_cluster_s32(mapa(saddr(&sm.failed), p)) != 0;
+        }
+        // sum over the shares of K in rank order, then the operator's own arithmetic, in place
+        for (int r = r0 + ew; r < r0 + share; r += kDrainWarps) {
+            const int row = m0 + r;
+#pragma unroll
+            for (int j = 0; j < kBN / 128; ++j) {
+                const int c = 128 * j + 4 * lane, col = n0 + c;
+                float4 v;
+                if (a.splits == 1) {
+                    v = *reinterpret_cast<const float4*>(tile + r * kTileLd + c);
+                } else {
+                    const uint32_t at = saddr(tile + r * kTileLd + c);
+                    v = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+                    for (int p = 0; p < a.splits; ++p) {
+                        const float4 q = ld_cluster_f4(mapa(at, PAIR ? 2 * p + half : p));
+                        v.x += q.x;
+                        v.y += q.y;
+                        v.z += q.z;
+                        v.w += q.w;
+                    }
+                }
+                v.x *= a.scale;
+                v.y *= a.scale;
+                v.z *= a.scale;
+                v.w *= a.scale;
+                if constexpr (KIND == kPoly) {
+                    if (row < a.m && col < a.ld) {
+                        const __half* src = a.A + (task * 2 * a.m + row) * a.ld + col;
+                        const uint2 h = *reinterpret_cast<const uint2*>(src);
+                        const uint2 l = *reinterpret_cast<const uint2*>(src + a.m * a.ld);
+                        const float2 h0 = __half22float2(*reinterpret_cast<const __half2*>(&h.x));
+                        const float2 h1 = __half22float2(*reinterpret_cast<const __half2*>(&h.y));
+                        const float2 l0 = __half22float2(*reinterpret_cast<const __half2*>(&l.x));
+                        const float2 l1 = __half22float2(*reinterpret_cast<const __half2*>(&l.y));
+                        v.x = fmaf(a.b, h0.x + l0.x, v.x) + (row == col ? a.a : 0.0f);
+                        v.y = fmaf(a.b, h0.y + l0.y, v.y) + (row == col + 1 ? a.a : 0.0f);
+                        v.z = fmaf(a.b, h1.x + l1.x, v.z) + (row == col + 2 ? a.a : 0.0f);
+                        v.w = fmaf(a.b, h1.y + l1.y, v.w) + (row == col + 3 ? a.a : 0.0f);
+                    }
+                }
+                if constexpr (KIND != kLast) {
+                    if (row < a.m && col < a.ld) {
+                        __half* dst = a.D + (task * 2 * a.m + row) * a.ld + col;
+                        uint2 h, l;
+                        split_half2(v.x, v.y, h.x, l.x);
+                        split_half2(v.z, v.w, h.y, l.y);
+                        *reinterpret_cast<uint2*>(dst) = h;
+                        *reinterpret_cast<uint2*>(dst + a.m * a.ld) = l;
+                    }
+                }
+                if (KIND == kLast || mirror) *reinterpret_cast<float4*>(tile + r * kTileLd + c) = v;
+            }
+        }
+        if (KIND == kLast || mirror) drain_sync();
+        if constexpr (kSym) {
+            if (mirror) {
+                // eight rows of one column to a thread: 16 bytes of a row of the mirror image
+                for (int i = threadIdx.x - kDrainWarp0 * 32; i < kBN * (share / 8); i += kDrainThreads) {
+                    const int c = i % kBN, r = r0 + i / kBN * 8;
+                    const int row = n0 + c, col = m0 + r;  // of the mirror image
+                    if (row >= a.m || col >= a.ld) continue;
+                    float v[8];
+#pragma unroll
+                    for (int k = 0; k < 8; ++k) v[k] = tile[(r + k) * kTileLd + c];
+                    uint4 h, l;
+                    split_half2(v[0], v[1], h.x, l.x);
+                    split_half2(v[2], v[3], h.y, l.y);
+                    split_half2(v[4], v[5], h.z, l.z);
+                    split_half2(v[6], v[7], h.w, l.w);
+                    __half* dst = a.D + (task * 2 * a.m + row) * a.ld + col;
+                    *reinterpret_cast<uint4*>(dst) = h;
+                    *reinterpret_cast<uint4*>(dst + a.m * a.ld) = l;
+                }
+            }
+        }
+        if constexpr (KIND == kLast) {
+            T* out = static_cast<T*>(a.out) + task * a.m * a.n;
+            const int total = share * kBN;
+            for (int i = threadIdx.x - kDrainWarp0 * 32; i < total; i += kDrainThreads) {
+                // neighbouring threads on neighbouring elements of the output
+                const int r = r0 + (a.tall ? i % share : i / kBN), c = a.tall ? i / share : i % kBN;
+                const int64_t row = m0 + r, col = n0 + c;
+                if (row >= a.m || col >= a.n) continue;
+                const int64_t e = a.tall ? col * a.m + row : row * a.n + col;
+                float v = tile[r * kTileLd + c];
+                if (a.update) v = fmaf(-a.rate, v, a.keep * to_arith<float>(out[e]));
+                if (bad) v = __int_as_float(0x7fc00000);
+                out[e] = from_arith<T>(v);
+            }
+        }
+    }
+    tc_fence_before();
+    __syncthreads();
+    if (csize > 1) cluster_sync();  // no read of a peer's shared memory is outstanding
+    if (warp == 1) {
+        tc_fence_after();
+        if constexpr (PAIR)
+            asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(kTmemCols) : "memory");
+        else
+            asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(kTmemCols) : "memory");
+    }
+    if (tid == 0 && sm.failed) atomicExch(a.status, 1);
+}
+
+// Planes [task][2][rows][ld] as a 4-D map of their `cols` valid columns; box 64 columns x box_rows x both planes.
+bool plane_map(CUtensorMap* map, const __half* base, int64_t cols, int64_t rows, int64_t ld, int64_t ntasks,
+               int box_rows) {
+    auto fn = tensor_map_encoder();
+    if (fn == nullptr) return false;
+    const cuuint64_t dims[4] = {cuuint64_t(cols), cuuint64_t(rows), 2, cuuint64_t(ntasks)};
+    const cuuint64_t strides[3] = {cuuint64_t(ld) * 2, cuuint64_t(rows * ld) * 2, cuuint64_t(2 * rows * ld) * 2};
+    const cuuint32_t box[4] = {kBK, cuuint32_t(box_rows), 2, 1}, one[4] = {1, 1, 1, 1};
+    return fn(map, CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 4, const_cast<__half*>(base), dims, strides, box, one,
+              CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+              CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
+
+// How a product is cut: the shape of its tiles and the shares of K.
+struct Cut {
+    bool pair;
+    int splits;
+    int64_t tiles_m, tiles_n, units;
+};
+
+// The cut with the least estimated time, in clocks: waves of clusters over the
+// SMs times (blocks of K per share + what a tile costs besides).  A pair's
+// block takes its 12 MMAs of 128 clocks; a single CTA's 12 MMAs of 64 wait for
+// the same bytes, about 1000 clocks.
+Cut cut_product(int64_t m, int64_t n, int64_t nkb, int64_t ntasks, bool sym) {
+    Cut best{};
+    double least = 0.0;
+    for (const bool pair : {true, false}) {
+        const int64_t bt = pair ? 256 : 128, tm = (m + bt - 1) / bt, tn = (n + bt - 1) / bt;
+        const int64_t units = sym ? tm * (tm + 1) / 2 : tm * tn;
+        for (int splits = 1; splits <= (pair ? 4 : 8); splits *= 2) {
+            if (splits > 1 && nkb < 2 * splits) break;
+            const int csize = splits * (pair ? 2 : 1);
+            const int64_t at_once = std::max<int64_t>(1, sm_count() / csize);
+            const int64_t waves = (units * ntasks + at_once - 1) / at_once;
+            const double block = pair ? 1600.0 : 1000.0;
+            const double tile = 3000.0 + (pair ? 5000.0 : 2500.0) / splits + (splits > 1 ? 2500.0 : 0.0);
+            const double t = double(waves) * (double((nkb + splits - 1) / splits) * block + tile);
+            if (least == 0.0 || t < least) {
+                least = t;
+                best = Cut{pair, splits, tm, tn, units};
+            }
+        }
+    }
+    return best;
+}
+
+template <bool PAIR, int KIND, typename T>
+cudaError_t launch_gemm(const CUtensorMap& left, const CUtensorMap& right, const GemmArgs& args, int64_t ntasks,
+                        cudaStream_t stream) {
+    static std::atomic<uint64_t> attr{0};
+    const size_t smem = sizeof(GemmSmem) + 1024;
+    auto kernel = ortho_gemm_kernel<PAIR, KIND, T>;
+    cudaError_t e = set_smem_limit_once(attr, kernel, smem);
+    if (e != cudaSuccess) return e;
+    const int csize = args.splits * (PAIR ? 2 : 1);
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3(unsigned(int64_t(args.units) * ntasks * csize));
+    cfg.blockDim = dim3(kThreads);
+    cfg.dynamicSmemBytes = smem;
+    cfg.stream = stream;
+    cudaLaunchAttribute at[2];
+    at[0].id = cudaLaunchAttributeClusterDimension;
+    at[0].val.clusterDim.x = unsigned(csize);
+    at[0].val.clusterDim.y = at[0].val.clusterDim.z = 1;
+    at[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    at[1].val.programmaticStreamSerializationAllowed = 1;
+    cfg.attrs = at;
+    cfg.numAttrs = 2;
+    count_launch();
+    return cudaLaunchKernelEx(&cfg, kernel, left, right, args);
+}
+
+template <int KIND, typename T>
+cudaError_t launch_cut(const Cut& cut, const CUtensorMap& left, const CUtensorMap& right, GemmArgs args, int64_t ntasks,
+                       cudaStream_t stream) {
+    args.tiles_m = int32_t(cut.tiles_m);
+    args.tiles_n = int32_t(cut.tiles_n);
+    args.units = int32_t(cut.units);
+    args.splits = cut.splits;
+    return cut.pair ? launch_gemm<true, KIND, T>(left, right, args, ntasks, stream)
+                    : launch_gemm<false, KIND, T>(left, right, args, ntasks, stream);
+}
+
+// The largest power of two that keeps `bound` times it within 2^15 (binary16 ends at 65504).
+float scale_for(double bound) { return float(std::exp2(15.0 - std::ceil(std::log2(bound)))); }
+
+}  // namespace
+
+float ortho_x_scale(const OrthoStep& s) { return scale_for(s.x_max); }
+
+template <typename T>
+int ortho_products(const OrthoPlanes& p, const OrthoSteps& steps, T* out, bool tall, const OrthoUpdate* up, int* status,
+                   cudaStream_t stream) {
+    const int64_t m = p.m, n = p.n;
+    const int64_t kbn = (n + kBK - 1) / kBK, kbm = (m + kBK - 1) / kBK;
+    const Cut gram = cut_product(m, m, kbn, p.ntasks, true), poly = cut_product(m, m, kbm, p.ntasks, true),
+              apply = cut_product(m, n, kbm, p.ntasks, false);
+    for (const Cut& c : {gram, poly, apply})
+        if (c.units * p.ntasks > (int64_t(1) << 27)) return GLMB_ERR_TOO_LARGE;
+    CUtensorMap x_rows[2], x_cols[2], a_rows, b_rows;
+    for (int i = 0; i < 2; ++i)
+        if (!plane_map(&x_rows[i], p.X[i], n, m, p.ld_n, p.ntasks, 128) ||
+            !plane_map(&x_cols[i], p.X[i], n, m, p.ld_n, p.ntasks, 64))
+            return GLMB_ERR_UNSUPPORTED;
+    if (!plane_map(&a_rows, p.A, m, m, p.ld_m, p.ntasks, 128) || !plane_map(&b_rows, p.B, m, m, p.ld_m, p.ntasks, 128))
+        return GLMB_ERR_UNSUPPORTED;
+    for (int k = 0; k < steps.n; ++k) {
+        const OrthoStep& s = steps.step[k];
+        const float sx = ortho_x_scale(s), sa = scale_for(s.x_max * s.x_max), sb = scale_for(std::max(s.b_max, 1e-3));
+        const int cur = k & 1;
+        const bool last = k + 1 == steps.n;
+        GemmArgs g{};
+        g.status = status;
+        g.m = g.n = m;
+        g.nkb = int32_t(kbn);
+        g.scale = sa / (sx * sx);
+        g.D = p.A;
+        g.ld = p.ld_m;
+        cudaError_t e = launch_cut<kGram, float>(gram, x_rows[cur], x_rows[cur], g, p.ntasks, stream);
+        if (e != cudaSuccess) return int(e);
+        g.nkb = int32_t(kbm);
+        g.scale = s.c * sb / (sa * sa);
+        g.a = s.a * sb;
+        g.b = s.b * sb / sa;
+        g.A = p.A;
+        g.D = p.B;
+        if ((e = launch_cut<kPoly, float>(poly, a_rows, a_rows, g, p.ntasks, stream)) != cudaSuccess) return int(e);
+        g.n = n;
+        g.A = nullptr;
+        g.ld = p.ld_n;
+        if (!last) {
+            g.D = p.X[cur ^ 1];
+            g.scale = ortho_x_scale(steps.step[k + 1]) / (sb * sx);
+            e = launch_cut<kApply, float>(apply, b_rows, x_cols[cur], g, p.ntasks, stream);
+        } else {
+            g.D = nullptr;
+            g.scale = 1.0f / (sb * sx);
+            g.out = out;
+            g.tall = tall;
+            g.update = up != nullptr;
+            if (up != nullptr) {
+                g.keep = up->keep;
+                g.rate = up->rate;
+            }
+            e = launch_cut<kLast, T>(apply, b_rows, x_cols[cur], g, p.ntasks, stream);
+        }
+        if (e != cudaSuccess) return int(e);
+    }
+    return launch_status();
+}
+
+template int ortho_products<float>(const OrthoPlanes&, const OrthoSteps&, float*, bool, const OrthoUpdate*, int*,
+                                   cudaStream_t);
+template int ortho_products<__half>(const OrthoPlanes&, const OrthoSteps&, __half*, bool, const OrthoUpdate*, int*,
+                                    cudaStream_t);
+template int ortho_products<__nv_bfloat16>(const OrthoPlanes&, const OrthoSteps&, __nv_bfloat16*, bool,
+                                           const OrthoUpdate*, int*, cudaStream_t);
+
+}  // namespace glmb
