@@ -165,7 +165,7 @@ size_t ortho_workspace(int64_t nf, int64_t nt, int64_t ntasks) {
     const int64_t m = std::min(nf, nt), n = std::max(nf, nt);
     if (m <= kOrthoSmallRows) return 0;
     return 256 + round_up(size_t(ntasks) * norm_blocks(m * n, ntasks) * 8, 256) +
-           2 * round_up(size_t(ntasks) * m * padded(n) * 4, 256) + 2 * round_up(size_t(ntasks) * m * padded(m) * 4, 256);
+           2 * round_up(size_t(ntasks) * m * padded(n) * 4, 256) + 3 * round_up(size_t(ntasks) * m * padded(m) * 4, 256);
 }
 
 template <typename T>
@@ -186,13 +186,14 @@ int ortho_run(const T* G, float* V, T* out, int64_t nf, int64_t nt, int64_t ntas
         w += round_up(bytes, 256);
         return p;
     };
-    OrthoPlanes p{m, n, padded(m), padded(n), ntasks, {}, nullptr, nullptr};
+    OrthoPlanes p{m, n, padded(m), padded(n), ntasks, {}, nullptr, nullptr, nullptr};
     int* status = reinterpret_cast<int*>(take(4));
     const int64_t nb = norm_blocks(size, ntasks);
     double* part = reinterpret_cast<double*>(take(size_t(ntasks) * nb * 8));
     for (__half*& x : p.X) x = reinterpret_cast<__half*>(take(size_t(ntasks) * m * p.ld_n * 4));
     p.A = reinterpret_cast<__half*>(take(size_t(ntasks) * m * p.ld_m * 4));
     p.B = reinterpret_cast<__half*>(take(size_t(ntasks) * m * p.ld_m * 4));
+    p.C = reinterpret_cast<__half*>(take(size_t(ntasks) * m * p.ld_m * 4));
     const OrthoUpdate up = update != nullptr ? *update : OrthoUpdate{};
     set_last_path("ortho_tensor");
     ortho_norm_kernel<T><<<dim3(unsigned(nb), unsigned(ntasks)), kThreads, 0, stream>>>(G, V, part, status, size, up);

@@ -35,6 +35,7 @@ struct OrthoPlanes {
     __half* X[2];  // m x n, before and after a step in turn
     __half* A;     // m x m
     __half* B;
+    __half* C;
 };
 // The power of two that X's planes carry before a step.
 float ortho_x_scale(const OrthoStep& s);

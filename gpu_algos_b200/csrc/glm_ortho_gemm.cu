@@ -1,6 +1,6 @@
 // glm_ortho_gemm.cu -- the three products of a Newton-Schulz step on the
 // 5th-generation tensor cores:
-//   A = X X^T,   B = aI + bA + cA A,   X' = B X      (X: m x n, m <= n).
+//   A = X X^T (and C = bI + cA),   B = aI + A C,   X' = B X      (X: m x n, m <= n).
 //
 // Operands are pairs of binary16 values, hi = the value rounded to nearest and
 // lo = the rest rounded to nearest, after a scaling by a power of two that the
@@ -40,6 +40,7 @@ constexpr int kBK = 64;   // K per stage: 128 bytes of binary16, one swizzle row
 constexpr int kStages = 3;
 constexpr int kPlaneBytes = 128 * kBK * 2;  // 128 rows (or columns) of one plane: 16 KB
 constexpr int kStageBytes = 4 * kPlaneBytes;  // left hi, lo, right hi, lo
+constexpr int kMaxSplits = 8;
 constexpr int kDrainWarp0 = 4, kDrainWarps = 8, kDrainThreads = kDrainWarps * 32;
 constexpr int kThreads = (kDrainWarp0 + kDrainWarps) * 32;
 // 384 threads launch with 168 registers each; the control warpgroup gives its share to the two that drain
@@ -122,6 +123,11 @@ __device__ __forceinline__ uint32_t mapa(uint32_t addr, uint32_t rank) {
     asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(r) : "r"(addr), "r"(rank));
     return r;
 }
+// Every thread of the cluster has come this far; nothing it wrote is published (a release waits for every
+// store in flight, about 2000 clocks behind a tile's output).  fence.mbarrier_init covers the barriers' set-up.
+__device__ __forceinline__ void cluster_sync_relaxed() {
+    asm volatile("barrier.cluster.arrive.relaxed.aligned;\n\tbarrier.cluster.wait.aligned;" ::: "memory");
+}
 __device__ __forceinline__ void drain_sync() { asm volatile("bar.sync 1, %0;" ::"n"(kDrainThreads) : "memory"); }
 
 __device__ __forceinline__ uint32_t pack_half2(float a, float b) {
@@ -136,6 +142,25 @@ __device__ __forceinline__ void split_half2(float a, float b, uint32_t& hi, uint
     lo = pack_half2(a - f.x, b - f.y);
 }
 
+// Four (eight) values at `hi` and their low parts a plane on.
+__device__ __forceinline__ void store_split4(__half* hi, int64_t plane, float4 v) {
+    uint2 h, l;
+    split_half2(v.x, v.y, h.x, l.x);
+    split_half2(v.z, v.w, h.y, l.y);
+    *reinterpret_cast<uint2*>(hi) = h;
+    *reinterpret_cast<uint2*>(hi + plane) = l;
+}
+__device__ __forceinline__ void store_split8(__half* hi, int64_t plane, const float (&v)[8]) {
+    uint4 h, l;
+    split_half2(v[0], v[1], h.x, l.x);
+    split_half2(v[2], v[3], h.y, l.y);
+    split_half2(v[4], v[5], h.z, l.z);
+    split_half2(v[6], v[7], h.w, l.w);
+    *reinterpret_cast<uint4*>(hi) = h;
+    *reinterpret_cast<uint4*>(hi + plane) = l;
+}
+
+// kGram: D = A = X X^T and D2 = C = bI + cA;  kPoly: D = B = aI + A C;  kApply: D = B X;  kLast: out from B X.
 enum : int { kGram, kPoly, kApply, kLast };
 
 struct GemmArgs {
@@ -145,9 +170,10 @@ struct GemmArgs {
     int32_t nkb;        // 64-deep blocks of K
     int32_t splits;     // CTAs (pairs) of a cluster, each with its share of K
     float scale;        // of the accumulated sum
-    float a, b;         // kPoly: on the diagonal, times A
-    const __half* A;    // kPoly: A's planes (D's layout)
+    float scale2;       // kGram: of D on its way to D2
+    float diag;         // on the diagonal of D2 (kGram) or D (kPoly)
     __half* D;          // planes [task][2][m][ld]
+    __half* D2;
     int64_t ld;
     void* out;          // kLast
     bool tall, update;
@@ -202,6 +228,8 @@ __global__ void __launch_bounds__(kThreads, 1)
     const int nkb = kb1 - kb0;
 
     if (tid == 0) {
+        asm volatile("prefetch.tensormap [%0];" ::"l"(&map_left) : "memory");
+        asm volatile("prefetch.tensormap [%0];" ::"l"(&map_right) : "memory");
         for (int s = 0; s < kStages; ++s) {
             mbar_init(&sm.full[s], 1);
             mbar_init(&sm.ready[s], 1);
@@ -230,7 +258,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     }
     tc_fence_before();
     __syncthreads();
-    cluster_sync();  // the peers' barriers exist before anyone arrives on them
+    if (csize > 1) cluster_sync_relaxed();  // the peers' barriers exist before anyone arrives on them
     tc_fence_after();
     const uint32_t tmem = sm.tmem_base;
     volatile int* failed = &sm.failed;
@@ -353,7 +381,6 @@ __global__ void __launch_bounds__(kThreads, 1)
     if (csize > 1) cluster_sync();  // the peers' partial tiles are complete
 
     if (warp >= kDrainWarp0) {
-        const int ew = warp - kDrainWarp0;
         const int share = kBM / a.splits;  // rows of the tile this CTA finishes
         const int r0 = int(part) * share;
         const bool mirror = kSym && ti != tj;
@@ -362,99 +389,108 @@ __global__ void __launch_bounds__(kThreads, 1)
             bad = *static_cast<volatile int*>(a.status) != 0;
             for (int p = 0; p < csize; ++p) bad |= ld_cluster_s32(mapa(saddr(&sm.failed), p)) != 0;
         }
-        // sum over the shares of K in rank order, then the operator's own arithmetic, in place
-        for (int r = r0 + ew; r < r0 + share; r += kDrainWarps) {
+        // Sum over the shares of K in rank order, scale, write; four columns to a thread.  The loops here are
+        // kept rolled: this code runs once per tile, and straight-line code costs an instruction fetch from L2
+        // every eight instructions.
+        const int dt = threadIdx.x - kDrainWarp0 * 32;
+        constexpr int kRowsAtOnce = kDrainThreads * 4 / kBN;
+        const int c = 4 * (dt % (kBN / 4)), col = n0 + c;
+#pragma unroll 2
+        for (int r = r0 + dt / (kBN / 4); r < r0 + share; r += kRowsAtOnce) {
             const int row = m0 + r;
+            float4 v;
+            if (a.splits == 1) {
+                v = *reinterpret_cast<const float4*>(tile + r * kTileLd + c);
+            } else {
+                const uint32_t at = saddr(tile + r * kTileLd + c);
+                float4 q[kMaxSplits];
 #pragma unroll
-            for (int j = 0; j < kBN / 128; ++j) {
-                const int c = 128 * j + 4 * lane, col = n0 + c;
-                float4 v;
-                if (a.splits == 1) {
-                    v = *reinterpret_cast<const float4*>(tile + r * kTileLd + c);
-                } else {
-                    const uint32_t at = saddr(tile + r * kTileLd + c);
-                    v = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-                    for (int p = 0; p < a.splits; ++p) {
-                        const float4 q = ld_cluster_f4(mapa(at, PAIR ? 2 * p + half : p));
-                        v.x += q.x;
-                        v.y += q.y;
-                        v.z += q.z;
-                        v.w += q.w;
+                for (int p = 0; p < kMaxSplits; ++p)
+                    if (p < a.splits) q[p] = ld_cluster_f4(mapa(at, PAIR ? 2 * p + half : p));
+                v = q[0];
+#pragma unroll
+                for (int p = 1; p < kMaxSplits; ++p)
+                    if (p < a.splits) {
+                        v.x += q[p].x;
+                        v.y += q[p].y;
+                        v.z += q[p].z;
+                        v.w += q[p].w;
                     }
-                }
-                v.x *= a.scale;
-                v.y *= a.scale;
-                v.z *= a.scale;
-                v.w *= a.scale;
-                if constexpr (KIND == kPoly) {
-                    if (row < a.m && col < a.ld) {
-                        const __half* src = a.A + (task * 2 * a.m + row) * a.ld + col;
-                        const uint2 h = *reinterpret_cast<const uint2*>(src);
-                        const uint2 l = *reinterpret_cast<const uint2*>(src + a.m * a.ld);
-                        const float2 h0 = __half22float2(*reinterpret_cast<const __half2*>(&h.x));
-                        const float2 h1 = __half22float2(*reinterpret_cast<const __half2*>(&h.y));
-                        const float2 l0 = __half22float2(*reinterpret_cast<const __half2*>(&l.x));
-                        const float2 l1 = __half22float2(*reinterpret_cast<const __half2*>(&l.y));
-                        v.x = fmaf(a.b, h0.x + l0.x, v.x) + (row == col ? a.a : 0.0f);
-                        v.y = fmaf(a.b, h0.y + l0.y, v.y) + (row == col + 1 ? a.a : 0.0f);
-                        v.z = fmaf(a.b, h1.x + l1.x, v.z) + (row == col + 2 ? a.a : 0.0f);
-                        v.w = fmaf(a.b, h1.y + l1.y, v.w) + (row == col + 3 ? a.a : 0.0f);
-                    }
-                }
-                if constexpr (KIND != kLast) {
-                    if (row < a.m && col < a.ld) {
-                        __half* dst = a.D + (task * 2 * a.m + row) * a.ld + col;
-                        uint2 h, l;
-                        split_half2(v.x, v.y, h.x, l.x);
-                        split_half2(v.z, v.w, h.y, l.y);
-                        *reinterpret_cast<uint2*>(dst) = h;
-                        *reinterpret_cast<uint2*>(dst + a.m * a.ld) = l;
-                    }
-                }
-                if (KIND == kLast || mirror) *reinterpret_cast<float4*>(tile + r * kTileLd + c) = v;
             }
+            v.x = fmaf(v.x, a.scale, KIND == kPoly && row == col ? a.diag : 0.0f);
+            v.y = fmaf(v.y, a.scale, KIND == kPoly && row == col + 1 ? a.diag : 0.0f);
+            v.z = fmaf(v.z, a.scale, KIND == kPoly && row == col + 2 ? a.diag : 0.0f);
+            v.w = fmaf(v.w, a.scale, KIND == kPoly && row == col + 3 ? a.diag : 0.0f);
+            if constexpr (KIND != kLast) {
+                if (row < a.m && col < a.ld) {
+                    const int64_t at = (task * 2 * a.m + row) * a.ld + col;
+                    store_split4(a.D + at, a.m * a.ld, v);
+                    if constexpr (KIND == kGram) {
+                        const float4 w = make_float4(
+                            fmaf(v.x, a.scale2, row == col ? a.diag : 0.0f),
+                            fmaf(v.y, a.scale2, row == col + 1 ? a.diag : 0.0f),
+                            fmaf(v.z, a.scale2, row == col + 2 ? a.diag : 0.0f),
+                            fmaf(v.w, a.scale2, row == col + 3 ? a.diag : 0.0f));
+                        store_split4(a.D2 + at, a.m * a.ld, w);
+                    }
+                }
+            }
+            if (KIND == kLast || mirror) *reinterpret_cast<float4*>(tile + r * kTileLd + c) = v;
         }
         if (KIND == kLast || mirror) drain_sync();
         if constexpr (kSym) {
             if (mirror) {
                 // eight rows of one column to a thread: 16 bytes of a row of the mirror image
-                for (int i = threadIdx.x - kDrainWarp0 * 32; i < kBN * (share / 8); i += kDrainThreads) {
+#pragma unroll 1
+                for (int i = dt; i < kBN * (share / 8); i += kDrainThreads) {
                     const int c = i % kBN, r = r0 + i / kBN * 8;
                     const int row = n0 + c, col = m0 + r;  // of the mirror image
                     if (row >= a.m || col >= a.ld) continue;
                     float v[8];
 #pragma unroll
                     for (int k = 0; k < 8; ++k) v[k] = tile[(r + k) * kTileLd + c];
-                    uint4 h, l;
-                    split_half2(v[0], v[1], h.x, l.x);
-                    split_half2(v[2], v[3], h.y, l.y);
-                    split_half2(v[4], v[5], h.z, l.z);
-                    split_half2(v[6], v[7], h.w, l.w);
-                    __half* dst = a.D + (task * 2 * a.m + row) * a.ld + col;
-                    *reinterpret_cast<uint4*>(dst) = h;
-                    *reinterpret_cast<uint4*>(dst + a.m * a.ld) = l;
+                    const int64_t at = (task * 2 * a.m + row) * a.ld + col;
+                    store_split8(a.D + at, a.m * a.ld, v);
+                    if constexpr (KIND == kGram) {
+#pragma unroll
+                        for (int k = 0; k < 8; ++k) v[k] *= a.scale2;  // off the diagonal
+                        store_split8(a.D2 + at, a.m * a.ld, v);
+                    }
                 }
             }
         }
         if constexpr (KIND == kLast) {
             T* out = static_cast<T*>(a.out) + task * a.m * a.n;
-            const int total = share * kBN;
-            for (int i = threadIdx.x - kDrainWarp0 * 32; i < total; i += kDrainThreads) {
-                // neighbouring threads on neighbouring elements of the output
-                const int r = r0 + (a.tall ? i % share : i / kBN), c = a.tall ? i / share : i % kBN;
-                const int64_t row = m0 + r, col = n0 + c;
-                if (row >= a.m || col >= a.n) continue;
-                const int64_t e = a.tall ? col * a.m + row : row * a.n + col;
-                float v = tile[r * kTileLd + c];
-                if (a.update) v = fmaf(-a.rate, v, a.keep * to_arith<float>(out[e]));
-                if (bad) v = __int_as_float(0x7fc00000);
-                out[e] = from_arith<T>(v);
+            const int share_log2 = 31 - __clz(share);
+            constexpr int kAhead = 8;  // share * kBN is a multiple of 8 * kDrainThreads
+#pragma unroll 1
+            for (int i0 = dt; i0 < share * kBN; i0 += kAhead * kDrainThreads) {
+                int64_t at[kAhead];
+                float v[kAhead], old[kAhead];
+#pragma unroll
+                for (int j = 0; j < kAhead; ++j) {
+                    // neighbouring threads on neighbouring elements of the output
+                    const int i = i0 + j * kDrainThreads;
+                    const int r = r0 + (a.tall ? i & (share - 1) : i / kBN), c = a.tall ? i >> share_log2 : i % kBN;
+                    const int64_t row = m0 + r, col = n0 + c;
+                    const bool in = row < a.m && col < a.n;
+                    at[j] = !in ? -1 : a.tall ? col * a.m + row : row * a.n + col;
+                    v[j] = tile[r * kTileLd + c];
+                    old[j] = a.update && in ? to_arith<float>(out[at[j]]) : 0.0f;
+                }
+#pragma unroll
+                for (int j = 0; j < kAhead; ++j) {
+                    if (at[j] < 0) continue;
+                    if (a.update) v[j] = fmaf(-a.rate, v[j], a.keep * old[j]);
+                    if (bad) v[j] = __int_as_float(0x7fc00000);
+                    out[at[j]] = from_arith<T>(v[j]);
+                }
             }
         }
     }
     tc_fence_before();
     __syncthreads();
-    if (csize > 1) cluster_sync();  // no read of a peer's shared memory is outstanding
+    if (csize > 1) cluster_sync_relaxed();  // no read of a peer's shared memory is outstanding
     if (warp == 1) {
         tc_fence_after();
         if constexpr (PAIR)
@@ -495,7 +531,7 @@ Cut cut_product(int64_t m, int64_t n, int64_t nkb, int64_t ntasks, bool sym) {
     for (const bool pair : {true, false}) {
         const int64_t bt = pair ? 256 : 128, tm = (m + bt - 1) / bt, tn = (n + bt - 1) / bt;
         const int64_t units = sym ? tm * (tm + 1) / 2 : tm * tn;
-        for (int splits = 1; splits <= (pair ? 4 : 8); splits *= 2) {
+        for (int splits = 1; splits <= (pair ? kMaxSplits / 2 : kMaxSplits); splits *= 2) {
             if (splits > 1 && nkb < 2 * splits) break;
             const int csize = splits * (pair ? 2 : 1);
             const int64_t at_once = std::max<int64_t>(1, sm_count() / csize);
@@ -550,7 +586,7 @@ cudaError_t launch_cut(const Cut& cut, const CUtensorMap& left, const CUtensorMa
 }
 
 // The largest power of two that keeps `bound` times it within 2^15 (binary16 ends at 65504).
-float scale_for(double bound) { return float(std::exp2(15.0 - std::ceil(std::log2(bound)))); }
+float scale_for(double bound) { return float(std::exp2(15.0 - std::ceil(std::log2(std::max(bound, 1e-3))))); }
 
 }  // namespace
 
@@ -565,16 +601,18 @@ int ortho_products(const OrthoPlanes& p, const OrthoSteps& steps, T* out, bool t
               apply = cut_product(m, n, kbm, p.ntasks, false);
     for (const Cut& c : {gram, poly, apply})
         if (c.units * p.ntasks > (int64_t(1) << 27)) return GLMB_ERR_TOO_LARGE;
-    CUtensorMap x_rows[2], x_cols[2], a_rows, b_rows;
+    CUtensorMap x_rows[2], x_cols[2], a_rows, b_rows, c_rows;
     for (int i = 0; i < 2; ++i)
         if (!plane_map(&x_rows[i], p.X[i], n, m, p.ld_n, p.ntasks, 128) ||
             !plane_map(&x_cols[i], p.X[i], n, m, p.ld_n, p.ntasks, 64))
             return GLMB_ERR_UNSUPPORTED;
-    if (!plane_map(&a_rows, p.A, m, m, p.ld_m, p.ntasks, 128) || !plane_map(&b_rows, p.B, m, m, p.ld_m, p.ntasks, 128))
+    if (!plane_map(&a_rows, p.A, m, m, p.ld_m, p.ntasks, 128) || !plane_map(&b_rows, p.B, m, m, p.ld_m, p.ntasks, 128) ||
+        !plane_map(&c_rows, p.C, m, m, p.ld_m, p.ntasks, 128))
         return GLMB_ERR_UNSUPPORTED;
     for (int k = 0; k < steps.n; ++k) {
         const OrthoStep& s = steps.step[k];
-        const float sx = ortho_x_scale(s), sa = scale_for(s.x_max * s.x_max), sb = scale_for(std::max(s.b_max, 1e-3));
+        const float sx = ortho_x_scale(s), sa = scale_for(s.x_max * s.x_max), sb = scale_for(s.b_max),
+                    sc = scale_for(std::fabs(s.b) + std::fabs(s.c) * s.x_max * s.x_max);
         const int cur = k & 1;
         const bool last = k + 1 == steps.n;
         GemmArgs g{};
@@ -582,19 +620,20 @@ int ortho_products(const OrthoPlanes& p, const OrthoSteps& steps, T* out, bool t
         g.m = g.n = m;
         g.nkb = int32_t(kbn);
         g.scale = sa / (sx * sx);
+        g.scale2 = s.c * sc / sa;
+        g.diag = s.b * sc;
         g.D = p.A;
+        g.D2 = p.C;
         g.ld = p.ld_m;
         cudaError_t e = launch_cut<kGram, float>(gram, x_rows[cur], x_rows[cur], g, p.ntasks, stream);
         if (e != cudaSuccess) return int(e);
         g.nkb = int32_t(kbm);
-        g.scale = s.c * sb / (sa * sa);
-        g.a = s.a * sb;
-        g.b = s.b * sb / sa;
-        g.A = p.A;
+        g.scale = sb / (sa * sc);
+        g.diag = s.a * sb;
         g.D = p.B;
-        if ((e = launch_cut<kPoly, float>(poly, a_rows, a_rows, g, p.ntasks, stream)) != cudaSuccess) return int(e);
+        g.D2 = nullptr;
+        if ((e = launch_cut<kPoly, float>(poly, a_rows, c_rows, g, p.ntasks, stream)) != cudaSuccess) return int(e);
         g.n = n;
-        g.A = nullptr;
         g.ld = p.ld_n;
         if (!last) {
             g.D = p.X[cur ^ 1];
