@@ -105,29 +105,6 @@ __device__ __forceinline__ void tma_load_4d(void* dst, const CUtensorMap* map, i
         : "memory");
 }
 
-__device__ __forceinline__ float4 ld_cluster_f4(uint32_t addr) {
-    float4 v;
-    asm volatile("ld.shared::cluster.v4.f32 {%0,%1,%2,%3}, [%4];"
-                 : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w)
-                 : "r"(addr)
-                 : "memory");
-    return v;
-}
-__device__ __forceinline__ int ld_cluster_s32(uint32_t addr) {
-    int v;
-    asm volatile("ld.shared::cluster.s32 %0, [%1];" : "=r"(v) : "r"(addr) : "memory");
-    return v;
-}
-__device__ __forceinline__ uint32_t mapa(uint32_t addr, uint32_t rank) {
-    uint32_t r;
-    asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(r) : "r"(addr), "r"(rank));
-    return r;
-}
-// Every thread of the cluster has come this far; nothing it wrote is published (a release waits for every
-// store in flight, about 2000 clocks behind a tile's output).  fence.mbarrier_init covers the barriers' set-up.
-__device__ __forceinline__ void cluster_sync_relaxed() {
-    asm volatile("barrier.cluster.arrive.relaxed.aligned;\n\tbarrier.cluster.wait.aligned;" ::: "memory");
-}
 __device__ __forceinline__ void drain_sync() { asm volatile("bar.sync 1, %0;" ::"n"(kDrainThreads) : "memory"); }
 
 __device__ __forceinline__ uint32_t pack_half2(float a, float b) {
@@ -387,7 +364,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         bool bad = false;
         if constexpr (KIND == kLast) {
             bad = *static_cast<volatile int*>(a.status) != 0;
-            for (int p = 0; p < csize; ++p) bad |= ld_cluster_s32(mapa(saddr(&sm.failed), p)) != 0;
+            for (int p = 0; p < csize; ++p) bad |= ld_cluster_s32(&sm.failed, p) != 0;
         }
         // Sum over the shares of K in rank order, scale, write; four columns to a thread.  The loops here are
         // kept rolled: this code runs once per tile, and straight-line code costs an instruction fetch from L2

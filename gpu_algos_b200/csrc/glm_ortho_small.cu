@@ -36,14 +36,6 @@ __device__ __forceinline__ void mma_f64(double (&d)[2], double a, double b) {
                  : "d"(a), "d"(b));
 }
 
-__device__ __forceinline__ double ld_cluster_f64(const double* p, uint32_t rank) {
-    uint32_t remote;
-    double v;
-    asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(remote) : "r"(saddr(p)), "r"(rank));
-    asm volatile("ld.shared::cluster.f64 %0, [%1];" : "=d"(v) : "r"(remote) : "memory");
-    return v;
-}
-
 template <int MT>
 struct SmallSmem {
     static constexpr int kM = 8 * MT, kLd = kM + 4;

@@ -8,6 +8,7 @@
 #include <algorithm>
 
 #include "glm_q4.cuh"
+#include "glm_tc.cuh"
 
 namespace glmb {
 
@@ -157,39 +158,277 @@ __global__ void __launch_bounds__(kThreads)
     }
 }
 
-// One warp per (task, 16 targets, observation).
+// ---- a few observations: the stream of the codes ------------------------------
+//
+// Bound by HBM: half a byte a weight, so with 1 to 32 observations the codes
+// are nearly all that moves.  A warp takes a block of 16 targets x 64 features
+// per step: one 16-byte load per lane is the block's four tensor-core
+// fragments (mma.m16n8k16, weights as the 16-row operand), made into whole
+// numbers of X's 16-bit type in registers, so a fragment costs the same for
+// one observation as for eight; products of 16-bit values are exact and sums
+// float.  A block's sums are scaled and added to the warp's totals.  float
+// observations are three bfloat16 terms (8 bits each, together all 24), each
+// with its own products.
+//
+// A CTA holds its observations' features in shared memory (in the order of
+// memory: lane 4g + c reads features 16c.. of observation g, which is what the
+// codes' order was chosen for); its eight warps share out row blocks and, where
+// a model has fewer than eight, features.  The features may also be shared by
+// the CTAs of a cluster, whose partial sums meet in distributed shared memory
+// in a fixed order.
+
+constexpr int kStreamChunk = 1024;  // features staged together
+constexpr int kStreamAhead = 4;     // blocks of codes in flight per warp
+
 template <typename T>
-__global__ void __launch_bounds__(kThreads)
-    q4_predict_kernel(const T* __restrict__ X, const uint4* __restrict__ codes, const T* __restrict__ scales,
-                      T* __restrict__ Yhat, int64_t nf, int64_t nt, int64_t ntasks, int64_t nrb, int64_t ncb,
-                      int64_t ngroups, int group, int64_t total, bool vec) {
-    const int lane = threadIdx.x & 31, g = lane >> 2, c = lane & 3;
-    for (int64_t w = int64_t(blockIdx.x) * kWarps + (threadIdx.x >> 5); w < total; w += int64_t(gridDim.x) * kWarps) {
-        const int64_t rb = w % nrb, task = w / nrb % ntasks, obs = w / nrb / ntasks;
-        const T* x = X + (obs * ntasks + task) * nf;
-        float acc[2] = {0.0f, 0.0f};
-        for (int64_t cb = 0; cb < ncb; ++cb) {
-            const uint4 block = codes[((task * nrb + rb) * ncb + cb) * 32 + lane];
-            const uint32_t word[4] = {block.x, block.y, block.z, block.w};
-            float v[16];
-            load16(x, cb * kQ4Cols + 16 * c, nf, vec, v);
-            const T* sc = scales + ((task * nrb + rb) * ngroups + cb * kQ4Cols / group) * kQ4Rows;
+struct Split16 {  // the 16-bit type the tensor core multiplies in, and how many terms an X takes
+    using Type = T;
+    static constexpr int kTerms = 1;
+};
+template <>
+struct Split16<float> {
+    using Type = __nv_bfloat16;
+    static constexpr int kTerms = 3;
+};
+
+template <typename H>
+__device__ __forceinline__ void mma_16816(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
+    if constexpr (std::is_same_v<H, __half>)
+        asm volatile(
+            "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+            : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+            : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+    else
+        asm volatile(
+            "mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+            : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+            : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+
+// The four pairs of a word of codes (u = q + 8) as 16-bit floats q: the code is put under the leading bit of
+// a power of two (1024 + u or, four bits up, 1024 + 16u in binary16; 128 + u in bfloat16) and the offset taken
+// off again, exactly.
+template <typename H>
+__device__ __forceinline__ void code_pairs(uint32_t w, uint32_t (&r)[4]) {
+    if constexpr (std::is_same_v<H, __half>) {
+        const __half2 off = __float2half2_rn(-1032.0f), sixteenth = __float2half2_rn(0.0625f),
+                      off16 = __float2half2_rn(-72.0f);
 #pragma unroll
-            for (int h = 0; h < 2; ++h) {
-                float d = 0.0f;
-#pragma unroll
-                for (int i = 0; i < 16; ++i) d = fmaf(float(code_of(word[i >> 2], (i & 2) + h, i & 1)), v[i], d);
-                acc[h] = fmaf(d, to_arith<float>(sc[g + 8 * h]), acc[h]);
-            }
+        for (int i = 0; i < 2; ++i) {
+            uint32_t lo = ((w >> (8 * i)) & 0x000f000fu) | 0x64006400u, hi = ((w >> (8 * i)) & 0x00f000f0u) | 0x64006400u;
+            const __half2 a = __hadd2(*reinterpret_cast<__half2*>(&lo), off);
+            const __half2 b = __hfma2(*reinterpret_cast<__half2*>(&hi), sixteenth, off16);
+            r[2 * i] = *reinterpret_cast<const uint32_t*>(&a);
+            r[2 * i + 1] = *reinterpret_cast<const uint32_t*>(&b);
         }
+    } else {
+        const __nv_bfloat162 off = __float2bfloat162_rn(-136.0f);
 #pragma unroll
-        for (int h = 0; h < 2; ++h) {
-            acc[h] += __shfl_xor_sync(0xffffffffu, acc[h], 1);
-            acc[h] += __shfl_xor_sync(0xffffffffu, acc[h], 2);
-            const int64_t t = rb * kQ4Rows + g + 8 * h;
-            if (c == 0 && t < nt) Yhat[(obs * ntasks + task) * nt + t] = from_arith<T>(acc[h]);
+        for (int i = 0; i < 4; ++i) {
+            uint32_t v = ((w >> (4 * i)) & 0x000f000fu) | 0x43004300u;
+            const __nv_bfloat162 a = __hadd2(*reinterpret_cast<__nv_bfloat162*>(&v), off);
+            r[i] = *reinterpret_cast<const uint32_t*>(&a);
         }
     }
+}
+
+// x as a sum of terms of the tensor core's type (one for a 16-bit x, three for a float)
+template <typename T>
+__device__ __forceinline__ void split_terms(T x, typename Split16<T>::Type (&t)[Split16<T>::kTerms]) {
+    if constexpr (std::is_same_v<T, float>) {
+        // a NaN or an infinity stays in the first term alone
+        t[0] = __float2bfloat16_rn(x);
+        const float r1 = x - __bfloat162float(t[0]);
+        const bool finite = fabsf(__bfloat162float(t[0])) <= 3.402823466e38f;
+        t[1] = __float2bfloat16_rn(finite ? r1 : 0.0f);
+        t[2] = __float2bfloat16_rn(finite ? r1 - __bfloat162float(t[1]) : 0.0f);
+    } else {
+        t[0] = x;
+    }
+}
+
+struct StreamArgs {
+    int64_t nf, nt, ntasks, nobs;
+    int64_t nrb, ncb, ngroups;
+    int64_t row_groups;   // CTAs (clusters) a task's row blocks take
+    int64_t per_rank;     // 64-feature blocks to a CTA of the cluster (even)
+    int group_log2;
+    int ranks;            // CTAs of a cluster, each with its share of the features
+    int rows_log2;        // log2 of the row blocks a CTA takes; 8 >> rows_log2 warps share each one's features
+    bool vec;
+};
+
+template <typename T, int NT>
+__global__ void __launch_bounds__(kThreads)
+    q4_stream_kernel(const T* __restrict__ X, const uint4* __restrict__ codes, const T* __restrict__ scales,
+                     T* __restrict__ Yhat, const StreamArgs a) {
+    using H = typename Split16<T>::Type;
+    constexpr int kTerms = Split16<T>::kTerms;
+    constexpr int kObs = 8 * NT;
+    constexpr int kRowBytes = kStreamChunk * 2 + 16;  // 16 past a multiple of 128: eight lanes' reads meet no bank twice
+    extern __shared__ __align__(16) unsigned char smem_raw[];
+    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, c = lane & 3;
+    const uint32_t rank = cluster_rank();
+    const int ranks = a.ranks;  // CTAs of a cluster
+    const int64_t unit = blockIdx.x / unsigned(ranks);
+    const int64_t rg = unit % a.row_groups, task = unit / a.row_groups % a.ntasks;
+    const int64_t obs0 = unit / a.row_groups / a.ntasks * kObs;
+    const int obs_here = int(min(int64_t(kObs), a.nobs - obs0));
+    const int rows = 1 << a.rows_log2, wk = warp >> a.rows_log2, wks = kWarps >> a.rows_log2;
+    const int64_t rb = rg * rows + (warp & (rows - 1));
+    const bool live = rb < a.nrb;
+    const int64_t cb_begin = int64_t(rank) * a.per_rank, cb_end = min(a.ncb, cb_begin + a.per_rank);
+    const uint4* my_codes = codes + ((task * a.nrb + (live ? rb : 0)) * a.ncb) * 32 + lane;
+    const T* my_scales = scales + (task * a.nrb + (live ? rb : 0)) * a.ngroups * kQ4Rows + g;
+
+    float total[NT][4] = {};
+    for (int64_t chunk = cb_begin; chunk < cb_end; chunk += kStreamChunk / kQ4Cols) {
+        const int blocks = int(min(int64_t(kStreamChunk / kQ4Cols), cb_end - chunk));
+        // this warp's blocks of the chunk: pairs of blocks wk, wk + wks, ...
+        const int pairs = (blocks + 1) / 2;
+        const int mine = live && pairs > wk ? 2 * ((pairs - wk + wks - 1) / wks) : 0;
+        uint4 w[kStreamAhead];
+        T s[kStreamAhead][2];
+        auto fetch = [&](int j, uint4& cw, T (&cs)[2]) {
+            const int b = 2 * ((j >> 1) * wks + wk) + (j & 1);
+            cw = make_uint4(0x88888888u, 0x88888888u, 0x88888888u, 0x88888888u);
+            cs[0] = cs[1] = from_arith<T>(0.0f);
+            if (j < mine && b < blocks) {
+                const int64_t cb = chunk + b;
+                asm volatile("ld.global.nc.L1::no_allocate.v4.u32 {%0,%1,%2,%3}, [%4];"
+                             : "=r"(cw.x), "=r"(cw.y), "=r"(cw.z), "=r"(cw.w)
+                             : "l"(my_codes + cb * 32));
+                const T* sc = my_scales + ((cb * kQ4Cols) >> a.group_log2) * kQ4Rows;
+                cs[0] = sc[0];
+                cs[1] = sc[8];
+            }
+        };
+#pragma unroll
+        for (int j = 0; j < kStreamAhead; ++j) fetch(j, w[j], s[j]);
+
+        if (chunk != cb_begin) __syncthreads();  // the chunk before has been read
+        {
+            constexpr int kPer = 16 / sizeof(T);
+            const int64_t f0 = chunk * kQ4Cols;
+            const int feats = blocks * kQ4Cols;
+            for (int i = tid; i < obs_here * (feats / kPer); i += kThreads) {
+                const int o = i / (feats / kPer), f = i % (feats / kPer) * kPer;
+                const T* src = X + ((obs0 + o) * a.ntasks + task) * a.nf + f0 + f;
+                T v[kPer] = {};
+                if (a.vec) {
+                    if (f0 + f < a.nf) VecLoad<T, kPer>::load(src, v);
+                } else {
+#pragma unroll
+                    for (int e = 0; e < kPer; ++e)
+                        if (f0 + f + e < a.nf) v[e] = src[e];
+                }
+                H t[kTerms][kPer];
+#pragma unroll
+                for (int e = 0; e < kPer; ++e) {
+                    H one[kTerms];
+                    split_terms<T>(v[e], one);
+#pragma unroll
+                    for (int q = 0; q < kTerms; ++q) t[q][e] = one[q];
+                }
+#pragma unroll
+                for (int q = 0; q < kTerms; ++q) {
+                    unsigned char* dst = smem_raw + (q * kObs + o) * kRowBytes + f * 2;
+                    if constexpr (kPer == 8) *reinterpret_cast<uint4*>(dst) = *reinterpret_cast<const uint4*>(t[q]);
+                    else *reinterpret_cast<uint2*>(dst) = *reinterpret_cast<const uint2*>(t[q]);
+                }
+            }
+        }
+        __syncthreads();
+
+        for (int j0 = 0; j0 < mine; j0 += kStreamAhead) {
+#pragma unroll
+            for (int jj = 0; jj < kStreamAhead; ++jj) {
+                const int j = j0 + jj;
+                const int b = 2 * ((j >> 1) * wks + wk) + (j & 1);
+                const uint4 cw = w[jj];
+                const float s0 = to_arith<float>(s[jj][0]), s1 = to_arith<float>(s[jj][1]);
+                fetch(j + kStreamAhead, w[jj], s[jj]);
+                if (j >= mine || b >= blocks) continue;
+                const uint32_t word[4] = {cw.x, cw.y, cw.z, cw.w};
+                uint32_t frag[4][4];
+#pragma unroll
+                for (int k = 0; k < 4; ++k) code_pairs<H>(word[k], frag[k]);
+#pragma unroll
+                for (int n = 0; n < NT; ++n) {
+                    // observations past the last one read another's row; their columns are not stored
+                    const int o = min(8 * n + g, obs_here - 1);
+                    float acc[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+                    for (int q = kTerms - 1; q >= 0; --q) {
+                        const uint4* x = reinterpret_cast<const uint4*>(smem_raw + (q * kObs + o) * kRowBytes +
+                                                                        (b * kQ4Cols + 16 * c) * 2);
+                        const uint4 x0 = x[0], x1 = x[1];
+                        mma_16816<H>(acc, frag[0], x0.x, x0.y);
+                        mma_16816<H>(acc, frag[1], x0.z, x0.w);
+                        mma_16816<H>(acc, frag[2], x1.x, x1.y);
+                        mma_16816<H>(acc, frag[3], x1.z, x1.w);
+                    }
+                    total[n][0] = fmaf(s0, acc[0], total[n][0]);
+                    total[n][1] = fmaf(s0, acc[1], total[n][1]);
+                    total[n][2] = fmaf(s1, acc[2], total[n][2]);
+                    total[n][3] = fmaf(s1, acc[3], total[n][3]);
+                }
+            }
+        }
+    }
+
+    // ---- the warps' and the cluster's partial sums ----
+    __syncthreads();
+    constexpr int kPartLd = kQ4Rows + 1;
+    float* part = reinterpret_cast<float*>(smem_raw);  // [warp][obs][16 targets]
+#pragma unroll
+    for (int n = 0; n < NT; ++n)
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+            part[(warp * kObs + 8 * n + 2 * c + (i & 1)) * kPartLd + g + 8 * (i >> 1)] = total[n][i];
+    __syncthreads();
+    if (ranks > 1) cluster_sync();
+    const int outputs = rows * kQ4Rows * obs_here;
+    const int begin = outputs * int(rank) / ranks, end = outputs * (int(rank) + 1) / ranks;
+    for (int i = begin + tid; i < end; i += kThreads) {
+        const int o = i / (rows * kQ4Rows), t = i % (rows * kQ4Rows);
+        const int64_t target = rg * rows * kQ4Rows + t;
+        float v = 0.0f;
+        for (int r = 0; r < ranks; ++r)
+            for (int k = 0; k < wks; ++k) {
+                const float* at = part + ((k * rows + t / kQ4Rows) * kObs + o) * kPartLd + t % kQ4Rows;
+                v += ranks > 1 ? ld_cluster_f32(at, r) : *at;
+            }
+        if (target < a.nt) Yhat[((obs0 + o) * a.ntasks + task) * a.nt + target] = from_arith<T>(v);
+    }
+    if (ranks > 1) cluster_sync_relaxed();  // the peers have read this CTA's sums
+}
+
+template <typename T, int NT>
+int stream_launch(const T* X, const void* codes, const T* scales, T* Yhat, const StreamArgs& a,
+                  cudaStream_t stream) {
+    const size_t smem = std::max(size_t(Split16<T>::kTerms) * 8 * NT * (kStreamChunk * 2 + 16),
+                                 size_t(kWarps) * 8 * NT * (kQ4Rows + 1) * 4);
+    static std::atomic<uint64_t> attr{0};
+    auto kernel = q4_stream_kernel<T, NT>;
+    cudaError_t e = set_smem_limit_once(attr, kernel, smem);
+    if (e != cudaSuccess) return int(e);
+    cudaLaunchConfig_t cfg = {};
+    const int64_t units = a.row_groups * a.ntasks * ((a.nobs + 8 * NT - 1) / (8 * NT));
+    if (units > (int64_t(1) << 31) / a.ranks - 1) return GLMB_ERR_TOO_LARGE;
+    cfg.gridDim = dim3(unsigned(units * a.ranks));
+    cfg.blockDim = dim3(kThreads);
+    cfg.dynamicSmemBytes = smem;
+    cfg.stream = stream;
+    cudaLaunchAttribute at[1];
+    at[0].id = cudaLaunchAttributeClusterDimension;
+    at[0].val.clusterDim.x = unsigned(a.ranks);
+    at[0].val.clusterDim.y = at[0].val.clusterDim.z = 1;
+    cfg.attrs = at;
+    cfg.numAttrs = 1;
+    count_launch();
+    e = cudaLaunchKernelEx(&cfg, kernel, X, static_cast<const uint4*>(codes), scales, Yhat, a);
+    return e != cudaSuccess ? int(e) : launch_status();
 }
 
 template <typename T>
@@ -231,12 +470,19 @@ template <typename T>
 int q4_predict(const T* X, const void* codes, const T* scales, T* Yhat, int64_t nf, int64_t nt, int64_t ntasks,
                int64_t nobs, int group, void*, size_t, cudaStream_t stream) {
     const int64_t nrb = q4_row_blocks(nt), ncb = q4_col_blocks(nf), ng = q4_groups(nf, group);
-    const int64_t total = ntasks * nrb * nobs;
-    q4_predict_kernel<T><<<warp_grid(total), kThreads, 0, stream>>>(X, static_cast<const uint4*>(codes), scales, Yhat,
-                                                                    nf, nt, ntasks, nrb, ncb, ng, group, total,
-                                                                    whole_vectors(X, nf));
-    count_launch();
-    return launch_status();
+    StreamArgs a{nf, nt, ntasks, nobs, nrb, ncb, ng, 0, 0, group == 64 ? 6 : 7, 1, 0, whole_vectors(X, nf)};
+    while (a.rows_log2 < 3 && (int64_t(1) << a.rows_log2) < nrb) ++a.rows_log2;
+    a.row_groups = (nrb + (int64_t(1) << a.rows_log2) - 1) >> a.rows_log2;
+    // CTAs that share a row group's features: until every SM has four CTAs, while each keeps 128 features a warp
+    const int64_t least = 2 * (kWarps >> a.rows_log2);
+    while (a.ranks < 8 && a.row_groups * ntasks * a.ranks * 2 <= 4 * int64_t(sm_count()) &&
+           ncb >= 2 * a.ranks * least)
+        a.ranks *= 2;
+    a.per_rank = ((ncb + a.ranks - 1) / a.ranks + 1) / 2 * 2;
+    set_last_path("q4_stream");
+    if (nobs <= 8) return stream_launch<T, 1>(X, codes, scales, Yhat, a, stream);
+    if (nobs <= 16) return stream_launch<T, 2>(X, codes, scales, Yhat, a, stream);
+    return stream_launch<T, 4>(X, codes, scales, Yhat, a, stream);
 }
 
 #define GLMB_INSTANTIATE_Q4(T)                                                                                \

@@ -108,6 +108,41 @@ __device__ __forceinline__ void reg_after(uint32_t (&r)[16]) {
                    "+r"(r[15]));
 }
 
+// Every thread of the cluster has come this far; nothing it wrote is published (a release waits for every
+// store in flight, about 2000 clocks behind a tile's output).
+__device__ __forceinline__ void cluster_sync_relaxed() {
+    asm volatile("barrier.cluster.arrive.relaxed.aligned;\n\tbarrier.cluster.wait.aligned;" ::: "memory");
+}
+// The address in CTA `rank` of this cluster of what is at `addr` here, and loads from there.
+__device__ __forceinline__ uint32_t mapa(uint32_t addr, uint32_t rank) {
+    uint32_t r;
+    asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(r) : "r"(addr), "r"(rank));
+    return r;
+}
+__device__ __forceinline__ float ld_cluster_f32(const float* p, uint32_t rank) {
+    float v;
+    asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(v) : "r"(mapa(saddr(p), rank)) : "memory");
+    return v;
+}
+__device__ __forceinline__ double ld_cluster_f64(const double* p, uint32_t rank) {
+    double v;
+    asm volatile("ld.shared::cluster.f64 %0, [%1];" : "=d"(v) : "r"(mapa(saddr(p), rank)) : "memory");
+    return v;
+}
+__device__ __forceinline__ int ld_cluster_s32(const int* p, uint32_t rank) {
+    int v;
+    asm volatile("ld.shared::cluster.s32 %0, [%1];" : "=r"(v) : "r"(mapa(saddr(p), rank)) : "memory");
+    return v;
+}
+__device__ __forceinline__ float4 ld_cluster_f4(uint32_t addr) {
+    float4 v;
+    asm volatile("ld.shared::cluster.v4.f32 {%0,%1,%2,%3}, [%4];"
+                 : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w)
+                 : "r"(addr)
+                 : "memory");
+    return v;
+}
+
 // cuTensorMapEncodeTiled, fetched through the runtime; nullptr without a driver (glm_dense.cu).
 PFN_cuTensorMapEncodeTiled_v12000 tensor_map_encoder();
 
