@@ -21,81 +21,130 @@ inline unsigned warp_grid(int64_t warps) {
     return unsigned(std::max<int64_t>(1, std::min<int64_t>(int64_t(sm_count()) * 32, (warps + kWarps - 1) / kWarps)));
 }
 
-// Sixteen consecutive features f0.. of one row (nullptr: a row past the last
-// target) as floats, zero past nf.  `vec`: rows start on 16 bytes and nf is a
-// whole number of 16-byte pieces, so a piece is inside or outside as a whole.
+// ---- rows of sixteen features -------------------------------------------------
+//
+// Lane 4g + c of a warp works on features 16c..16c+15 of a 64-feature block of
+// rows g and g + 8.  Where rows start on 16 bytes (`vec`) it moves its sixteen
+// as 16-byte pieces; elsewhere the warp moves each row's 64 features side by
+// side and passes them through shared memory.
+
+constexpr int kTileLd = kQ4Cols + 8;  // elements of T between the rows of a staged block
+
 template <typename T>
-__device__ __forceinline__ void load16(const T* row, int64_t f0, int64_t nf, bool vec, float (&v)[16]) {
+struct RowTile {
+    alignas(16) T at[kQ4Rows][kTileLd];
+};
+
+// v = features f0 + 16c.. of rows row0 + g and row0 + g + 8 (zero past nf and past `rows`) of M[.][nf].
+template <typename T>
+__device__ __forceinline__ void load_rows(const T* M, int64_t row0, int rows, int64_t f0, int64_t nf, bool vec,
+                                          RowTile<T>& tile, float (&v)[2][16]) {
     constexpr int kPer = 16 / sizeof(T);
+    const int lane = threadIdx.x & 31, g = lane >> 2, c = lane & 3;
     if (vec) {
 #pragma unroll
-        for (int i = 0; i < 16; i += kPer) {
-            T t[kPer] = {};
-            if (row != nullptr && f0 + i < nf) VecLoad<T, kPer>::load(row + f0 + i, t);
+        for (int h = 0; h < 2; ++h)
 #pragma unroll
-            for (int j = 0; j < kPer; ++j) v[i + j] = to_arith<float>(t[j]);
-        }
+            for (int i = 0; i < 16; i += kPer) {
+                T t[kPer] = {};
+                if (g + 8 * h < rows && f0 + 16 * c + i < nf)
+                    VecLoad<T, kPer>::load(M + (row0 + g + 8 * h) * nf + f0 + 16 * c + i, t);
+#pragma unroll
+                for (int j = 0; j < kPer; ++j) v[h][i + j] = to_arith<float>(t[j]);
+            }
     } else {
+        __syncwarp();
+#pragma unroll 4
+        for (int r = 0; r < kQ4Rows; ++r)
 #pragma unroll
-        for (int i = 0; i < 16; ++i) v[i] = row != nullptr && f0 + i < nf ? to_arith<float>(row[f0 + i]) : 0.0f;
+            for (int i = 0; i < 2; ++i) {
+                const int64_t f = f0 + lane + 32 * i;
+                tile.at[r][lane + 32 * i] = r < rows && f < nf ? M[(row0 + r) * nf + f] : from_arith<T>(0.0f);
+            }
+        __syncwarp();
+#pragma unroll
+        for (int h = 0; h < 2; ++h)
+#pragma unroll
+            for (int i = 0; i < 16; i += kPer) {
+                alignas(16) T t[kPer];
+                *reinterpret_cast<uint4*>(t) = *reinterpret_cast<const uint4*>(&tile.at[g + 8 * h][16 * c + i]);
+#pragma unroll
+                for (int j = 0; j < kPer; ++j) v[h][i + j] = to_arith<float>(t[j]);
+            }
     }
 }
 
-// w / s rounded to the nearest whole number, ties to even, within -7..7, for
-// |w| <= 7.5 s or so and s > 0.  The float product w * (1/s) can be off by an
-// ulp and land on the wrong side of a border, so the remainder w - r*s decides:
-// it is exact in float (w and r*s are multiples of ulp(s)/2 when r != 0 and
-// the remainder is about s/2 at most).
-__device__ __forceinline__ int nearest_code(float w, float s, float inv) {
-    float r = fminf(fmaxf(rintf(w * inv), -7.0f), 7.0f);
-    const float d = fmaf(-r, s, w), half = 0.5f * s;
-    const bool odd = (int(r) & 1) != 0;
-    if (fabsf(d) > half || (fabsf(d) == half && odd)) r += d > 0.0f ? 1.0f : -1.0f;
-    return int(fminf(fmaxf(r, -7.0f), 7.0f));
+__device__ __forceinline__ float max_abs_nan(float a, float b) {
+    float r;
+    asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(fabsf(b)));
+    return r;
 }
 
-// One warp per (task, 16 targets, group): lane 4g + c takes features 16c..16c+15
-// of each 64-feature block of targets g and g + 8, so the group's largest
-// magnitude is a maximum over the four lanes of a target.  One pass, bound by
-// HBM: the weights in, codes and scales out.
+// q + 8 with q = w / s rounded to the nearest whole number, ties to even, for |w / s| < 7.5 and s > 0.  The
+// float product w * (1/s) can be off by an ulp and land on the wrong side of a border, so the remainder
+// d = w - q*s decides: it is exact in float (w and q*s are multiples of ulp(s)/2 when q != 0, and |d| is s/2
+// or so).  `half` is s/2 and `below` the next float towards zero, the limits for even and for odd q.
+__device__ __forceinline__ uint32_t nearest_code(float w, float s, float inv, float half, float below) {
+    constexpr float kOne = 12582912.0f;  // 1.5 * 2^23: adding it rounds to a whole number, found in the low bits
+    const float m = fmaf(w, inv, kOne);
+    const float d = fmaf(kOne - m, s, w);
+    const int bits = __float_as_int(m);
+    const int step = (__float_as_int(d) >> 31) | 1;
+    return uint32_t(bits + 8 + (fabsf(d) > ((bits & 1) != 0 ? below : half) ? step : 0)) & 15u;
+}
+
+// One warp per (task, 16 targets, group).  A group's largest magnitude is a maximum over the four lanes of
+// a target.  One pass: the weights in, codes and scales out.
 template <typename T, int GROUP>
 __global__ void __launch_bounds__(kThreads)
     q4_quantize_kernel(const T* __restrict__ M, uint4* __restrict__ codes, T* __restrict__ scales, int64_t nf,
                        int64_t nt, int64_t nrb, int64_t ncb, int64_t ngroups, int64_t total, bool vec) {
     constexpr int kBlocks = GROUP / kQ4Cols;
-    const int lane = threadIdx.x & 31, g = lane >> 2, c = lane & 3;
-    for (int64_t w = int64_t(blockIdx.x) * kWarps + (threadIdx.x >> 5); w < total; w += int64_t(gridDim.x) * kWarps) {
+    __shared__ RowTile<T> tiles[kWarps];
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, c = lane & 3;
+    for (int64_t w = int64_t(blockIdx.x) * kWarps + warp; w < total; w += int64_t(gridDim.x) * kWarps) {
         const int64_t group = w % ngroups, rb = w / ngroups % nrb, task = w / ngroups / nrb;
-        float v[2][kBlocks][16];
-        float s[2], inv[2], up[2];
+        const int rows = int(min(int64_t(kQ4Rows), nt - rb * kQ4Rows));
+        float v[kBlocks][2][16];
+#pragma unroll
+        for (int b = 0; b < kBlocks; ++b)
+            load_rows(M, task * nt + rb * kQ4Rows, rows, group * GROUP + b * kQ4Cols, nf, vec, tiles[warp], v[b]);
+        float s[2], inv[2];
+        T st[2];
 #pragma unroll
         for (int h = 0; h < 2; ++h) {
-            const int64_t t = rb * kQ4Rows + g + 8 * h;
-            const T* row = t < nt ? M + (task * nt + t) * nf : nullptr;
             float top = 0.0f;
-            bool bad = false;
 #pragma unroll
-            for (int b = 0; b < kBlocks; ++b) {
-                load16(row, group * GROUP + b * kQ4Cols + 16 * c, nf, vec, v[h][b]);
+            for (int b = 0; b < kBlocks; ++b)
 #pragma unroll
-                for (int i = 0; i < 16; ++i) {
-                    top = fmaxf(top, fabsf(v[h][b][i]));
-                    bad |= !(fabsf(v[h][b][i]) <= 3.402823466e38f);
-                }
+                for (int i = 0; i < 16; ++i) top = max_abs_nan(top, v[b][h][i]);
+#pragma unroll
+            for (int off = 1; off < 4; off <<= 1) top = max_abs_nan(top, __shfl_xor_sync(0xffffffffu, top, off));
+            const bool finite = top <= 3.402823466e38f;
+            st[h] = from_arith<T>(finite ? __fdiv_rn(top, 7.0f) : __int_as_float(0x7fc00000));
+            s[h] = finite ? to_arith<float>(st[h]) : 0.0f;
+            if (s[h] < 0x1p-100f || top > 7.25f * s[h]) {
+                // Rare: a group of zeros or with a NaN (every code is 0); a scale near the bottom of float's
+                // range, lifted with its weights, which changes no ratio; one rounded so far down, among the
+                // subnormals of T, that weights reach past 7.
+                const float up = s[h] < 0x1p-100f ? 0x1p60f : 1.0f;
+                const float most = 7.0f * (s[h] * up);
+#pragma unroll
+                for (int b = 0; b < kBlocks; ++b)
+#pragma unroll
+                    for (int i = 0; i < 16; ++i)
+                        v[b][h][i] = s[h] > 0.0f ? fminf(fmaxf(v[b][h][i] * up, -most), most) : 0.0f;
+                s[h] = s[h] > 0.0f ? s[h] * up : 1.0f;
             }
-#pragma unroll
-            for (int off = 1; off < 4; off <<= 1) {
-                top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, off));
-                bad |= __shfl_xor_sync(0xffffffffu, int(bad), off) != 0;
-            }
-            const T st = from_arith<T>(bad ? __int_as_float(0x7fc00000) : __fdiv_rn(top, 7.0f));
-            if (c == 0) scales[((task * nrb + rb) * ngroups + group) * kQ4Rows + g + 8 * h] = st;
-            const float sf = to_arith<float>(st);
-            // scales near the bottom of float's range are lifted with their weights, which changes no ratio
-            up[h] = sf < 0x1p-100f ? 0x1p60f : 1.0f;
-            s[h] = bad ? 0.0f : sf * up[h];
-            inv[h] = s[h] > 0.0f ? __frcp_rn(s[h]) : 0.0f;
+            inv[h] = __frcp_rn(s[h]);
         }
+        if (c == 0) {
+            T* dst = scales + ((task * nrb + rb) * ngroups + group) * kQ4Rows + 2 * g;
+            dst[0] = st[0];
+            dst[1] = st[1];
+        }
+        const float half[2] = {0.5f * s[0], 0.5f * s[1]};
+        const float below[2] = {__int_as_float(__float_as_int(half[0]) - 1), __int_as_float(__float_as_int(half[1]) - 1)};
 #pragma unroll
         for (int b = 0; b < kBlocks; ++b) {
             const int64_t cb = group * kBlocks + b;
@@ -108,8 +157,7 @@ __global__ void __launch_bounds__(kThreads)
                 for (int p = 0; p < 8; ++p) {
                     // p: pair 0..3 = (g, f), (g+8, f), (g, f+2), (g+8, f+2); 4..7 the same of f + 1
                     const int h = p & 1, i = 4 * k + (p & 2) + (p >> 2);
-                    const int q = s[h] > 0.0f ? nearest_code(v[h][b][i] * up[h], s[h], inv[h]) : 0;
-                    word[k] |= uint32_t(q + 8) << (4 * (p & 3) + 16 * (p >> 2));
+                    word[k] |= nearest_code(v[b][h][i], s[h], inv[h], half[h], below[h]) << (4 * (p & 3) + 16 * (p >> 2));
                 }
             }
             codes[((task * nrb + rb) * ncb + cb) * 32 + lane] = make_uint4(word[0], word[1], word[2], word[3]);
@@ -117,71 +165,9 @@ __global__ void __launch_bounds__(kThreads)
     }
 }
 
-// The code (q) of pair p (0..3), first or second element, of a word.
-__device__ __forceinline__ int code_of(uint32_t word, int p, int second) {
-    return int((word >> (4 * p + 16 * second)) & 15u) - 8;
-}
-
-// One warp per block of codes: M = q*s (exact in float), rounded to T.
+// The 16-bit type the tensor core multiplies in, and how many terms an X takes.
 template <typename T>
-__global__ void __launch_bounds__(kThreads)
-    q4_dequantize_kernel(const uint4* __restrict__ codes, const T* __restrict__ scales, T* __restrict__ M, int64_t nf,
-                         int64_t nt, int64_t nrb, int64_t ncb, int64_t ngroups, int group, int64_t total, bool vec) {
-    constexpr int kPer = 16 / sizeof(T);
-    const int lane = threadIdx.x & 31, g = lane >> 2, c = lane & 3;
-    for (int64_t w = int64_t(blockIdx.x) * kWarps + (threadIdx.x >> 5); w < total; w += int64_t(gridDim.x) * kWarps) {
-        const int64_t cb = w % ncb, rb = w / ncb % nrb, task = w / ncb / nrb;
-        const uint4 block = codes[w * 32 + lane];
-        const uint32_t word[4] = {block.x, block.y, block.z, block.w};
-        const int64_t f0 = cb * kQ4Cols + 16 * c;
-        const T* sc = scales + ((task * nrb + rb) * ngroups + cb * kQ4Cols / group) * kQ4Rows;
-#pragma unroll
-        for (int h = 0; h < 2; ++h) {
-            const int64_t t = rb * kQ4Rows + g + 8 * h;
-            if (t >= nt) continue;
-            const float s = to_arith<float>(sc[g + 8 * h]);
-            T* row = M + (task * nt + t) * nf + f0;
-            alignas(16) T out[16];
-#pragma unroll
-            for (int i = 0; i < 16; ++i)
-                out[i] = from_arith<T>(float(code_of(word[i >> 2], (i & 2) + h, i & 1)) * s);
-            if (vec) {
-#pragma unroll
-                for (int i = 0; i < 16; i += kPer)
-                    if (f0 + i < nf) *reinterpret_cast<uint4*>(row + i) = *reinterpret_cast<const uint4*>(out + i);
-            } else {
-#pragma unroll
-                for (int i = 0; i < 16; ++i)
-                    if (f0 + i < nf) row[i] = out[i];
-            }
-        }
-    }
-}
-
-// ---- a few observations: the stream of the codes ------------------------------
-//
-// Bound by HBM: half a byte a weight, so with 1 to 32 observations the codes
-// are nearly all that moves.  A warp takes a block of 16 targets x 64 features
-// per step: one 16-byte load per lane is the block's four tensor-core
-// fragments (mma.m16n8k16, weights as the 16-row operand), made into whole
-// numbers of X's 16-bit type in registers, so a fragment costs the same for
-// one observation as for eight; products of 16-bit values are exact and sums
-// float.  A block's sums are scaled and added to the warp's totals.  float
-// observations are three bfloat16 terms (8 bits each, together all 24), each
-// with its own products.
-//
-// A CTA holds its observations' features in shared memory (in the order of
-// memory: lane 4g + c reads features 16c.. of observation g, which is what the
-// codes' order was chosen for); its eight warps share out row blocks and, where
-// a model has fewer than eight, features.  The features may also be shared by
-// the CTAs of a cluster, whose partial sums meet in distributed shared memory
-// in a fixed order.
-
-constexpr int kStreamChunk = 1024;  // features staged together
-constexpr int kStreamAhead = 4;     // blocks of codes in flight per warp
-
-template <typename T>
-struct Split16 {  // the 16-bit type the tensor core multiplies in, and how many terms an X takes
+struct Split16 {
     using Type = T;
     static constexpr int kTerms = 1;
 };
@@ -190,20 +176,6 @@ struct Split16<float> {
     using Type = __nv_bfloat16;
     static constexpr int kTerms = 3;
 };
-
-template <typename H>
-__device__ __forceinline__ void mma_16816(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
-    if constexpr (std::is_same_v<H, __half>)
-        asm volatile(
-            "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
-            : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
-            : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
-    else
-        asm volatile(
-            "mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
-            : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
-            : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
-}
 
 // The four pairs of a word of codes (u = q + 8) as 16-bit floats q: the code is put under the leading bit of
 // a power of two (1024 + u or, four bits up, 1024 + 16u in binary16; 128 + u in bfloat16) and the offset taken
@@ -232,6 +204,114 @@ __device__ __forceinline__ void code_pairs(uint32_t w, uint32_t (&r)[4]) {
     }
 }
 
+// A pair of codes times a scale, rounded to T, as the 32-bit words of two elements of T (one for 16-bit types).
+template <typename T>
+__device__ __forceinline__ void scaled_pair(uint32_t pair, T s, uint32_t* dst) {
+    if constexpr (std::is_same_v<T, float>) {
+        dst[0] = __float_as_uint(__uint_as_float(pair << 16) * s);
+        dst[1] = __float_as_uint(__uint_as_float(pair & 0xffff0000u) * s);
+    } else if constexpr (std::is_same_v<T, __half>) {
+        const __half2 v = __hmul2(*reinterpret_cast<const __half2*>(&pair), __half2half2(s));
+        dst[0] = *reinterpret_cast<const uint32_t*>(&v);
+    } else {
+        const __nv_bfloat162 v = __hmul2(*reinterpret_cast<const __nv_bfloat162*>(&pair), __bfloat162bfloat162(s));
+        dst[0] = *reinterpret_cast<const uint32_t*>(&v);
+    }
+}
+
+// One warp per block of codes: M = q*s, rounded to T.
+template <typename T>
+__global__ void __launch_bounds__(kThreads)
+    q4_dequantize_kernel(const uint4* __restrict__ codes, const T* __restrict__ scales, T* __restrict__ M, int64_t nf,
+                         int64_t nt, int64_t nrb, int64_t ncb, int64_t ngroups, int group_log2, int64_t total, bool vec) {
+    using H = typename Split16<T>::Type;
+    constexpr int kWords = 16 * sizeof(T) / 4;  // of a lane's sixteen features of one row
+    __shared__ RowTile<T> tiles[kWarps];
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, c = lane & 3;
+    for (int64_t w = int64_t(blockIdx.x) * kWarps + warp; w < total; w += int64_t(gridDim.x) * kWarps) {
+        const int64_t cb = w % ncb, rb = w / ncb % nrb, task = w / ncb / nrb;
+        const uint4 block = codes[w * 32 + lane];
+        const T* sc = scales + ((task * nrb + rb) * ngroups + ((cb * kQ4Cols) >> group_log2)) * kQ4Rows + 2 * g;
+        const T s[2] = {sc[0], sc[1]};
+        const uint32_t word[4] = {block.x, block.y, block.z, block.w};
+        uint32_t out[2][kWords];
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+            uint32_t pair[4];
+            code_pairs<H>(word[k], pair);
+#pragma unroll
+            for (int p = 0; p < 4; ++p) scaled_pair<T>(pair[p], s[p & 1], &out[p & 1][(2 * k + (p >> 1)) * kWords / 8]);
+        }
+        const int rows = int(min(int64_t(kQ4Rows), nt - rb * kQ4Rows));
+        const int64_t row0 = task * nt + rb * kQ4Rows, f0 = cb * kQ4Cols;
+        if (vec) {
+#pragma unroll
+            for (int h = 0; h < 2; ++h) {
+                if (g + 8 * h >= rows) continue;
+                T* dst = M + (row0 + g + 8 * h) * nf + f0 + 16 * c;
+#pragma unroll
+                for (int i = 0; i < kWords; i += 4)
+                    if (f0 + 16 * c + i * int(4 / sizeof(T)) < nf)
+                        *reinterpret_cast<uint4*>(reinterpret_cast<uint32_t*>(dst) + i) =
+                            make_uint4(out[h][i], out[h][i + 1], out[h][i + 2], out[h][i + 3]);
+            }
+        } else {
+            RowTile<T>& tile = tiles[warp];
+            __syncwarp();
+#pragma unroll
+            for (int h = 0; h < 2; ++h)
+#pragma unroll
+                for (int i = 0; i < kWords; i += 4)
+                    *reinterpret_cast<uint4*>(reinterpret_cast<uint32_t*>(&tile.at[g + 8 * h][16 * c]) + i) =
+                        make_uint4(out[h][i], out[h][i + 1], out[h][i + 2], out[h][i + 3]);
+            __syncwarp();
+#pragma unroll 4
+            for (int r = 0; r < kQ4Rows; ++r)
+#pragma unroll
+                for (int i = 0; i < 2; ++i) {
+                    const int64_t f = f0 + lane + 32 * i;
+                    if (r < rows && f < nf) M[(row0 + r) * nf + f] = tile.at[r][lane + 32 * i];
+                }
+        }
+    }
+}
+
+// ---- a few observations: the stream of the codes ------------------------------
+//
+// Bound by HBM: half a byte a weight, so with 1 to 32 observations the codes
+// are nearly all that moves.  A warp takes a block of 16 targets x 64 features
+// per step: one 16-byte load per lane is the block's four tensor-core
+// fragments (mma.m16n8k16, weights as the 16-row operand), made into whole
+// numbers of X's 16-bit type in registers, so a fragment costs the same for
+// one observation as for eight; products of 16-bit values are exact and sums
+// float.  A block's sums are scaled and added to the warp's totals.  float
+// observations are three bfloat16 terms (8 bits each, together all 24), each
+// with its own products.
+//
+// A CTA holds its observations' features in shared memory (in the order of
+// memory: lane 4g + c reads features 16c.. of observation g, which is what the
+// codes' order was chosen for); its eight warps share out row blocks and, where
+// a model has fewer than eight, features.  The features may also be shared by
+// the CTAs of a cluster, whose partial sums meet in distributed shared memory
+// in a fixed order.
+
+constexpr int kStreamChunk = 1024;  // features staged together
+constexpr int kStreamAhead = 4;     // blocks of codes in flight per warp
+
+template <typename H>
+__device__ __forceinline__ void mma_16816(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
+    if constexpr (std::is_same_v<H, __half>)
+        asm volatile(
+            "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+            : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+            : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+    else
+        asm volatile(
+            "mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+            : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+            : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+
 // x as a sum of terms of the tensor core's type (one for a 16-bit x, three for a float)
 template <typename T>
 __device__ __forceinline__ void split_terms(T x, typename Split16<T>::Type (&t)[Split16<T>::kTerms]) {
@@ -246,6 +326,11 @@ __device__ __forceinline__ void split_terms(T x, typename Split16<T>::Type (&t)[
         t[0] = x;
     }
 }
+
+template <typename T>
+struct alignas(2 * sizeof(T)) Pair {
+    T first, second;
+};
 
 struct StreamArgs {
     int64_t nf, nt, ntasks, nobs;
@@ -279,32 +364,29 @@ __global__ void __launch_bounds__(kThreads)
     const bool live = rb < a.nrb;
     const int64_t cb_begin = int64_t(rank) * a.per_rank, cb_end = min(a.ncb, cb_begin + a.per_rank);
     const uint4* my_codes = codes + ((task * a.nrb + (live ? rb : 0)) * a.ncb) * 32 + lane;
-    const T* my_scales = scales + (task * a.nrb + (live ? rb : 0)) * a.ngroups * kQ4Rows + g;
+    const T* my_scales = scales + (task * a.nrb + (live ? rb : 0)) * a.ngroups * kQ4Rows + 2 * g;
+    const int group_shift = a.group_log2 - 6;
 
     float total[NT][4] = {};
     for (int64_t chunk = cb_begin; chunk < cb_end; chunk += kStreamChunk / kQ4Cols) {
         const int blocks = int(min(int64_t(kStreamChunk / kQ4Cols), cb_end - chunk));
-        // this warp's blocks of the chunk: pairs of blocks wk, wk + wks, ...
-        const int pairs = (blocks + 1) / 2;
-        const int mine = live && pairs > wk ? 2 * ((pairs - wk + wks - 1) / wks) : 0;
+        // (blocks come in pairs of 128 features: a warp's j-th is block wk2 + (j/2) * stride + j%2)
+        const int wk2 = 2 * wk, stride = 2 * wks;
+        const uint4* cp = my_codes + chunk * 32;
+        const T* sp = my_scales + ((chunk * kQ4Cols) >> a.group_log2) * kQ4Rows;
+        const int limit = live ? blocks : 0;
         uint4 w[kStreamAhead];
-        T s[kStreamAhead][2];
-        auto fetch = [&](int j, uint4& cw, T (&cs)[2]) {
-            const int b = 2 * ((j >> 1) * wks + wk) + (j & 1);
-            cw = make_uint4(0x88888888u, 0x88888888u, 0x88888888u, 0x88888888u);
-            cs[0] = cs[1] = from_arith<T>(0.0f);
-            if (j < mine && b < blocks) {
-                const int64_t cb = chunk + b;
+        Pair<T> s[kStreamAhead];
+        auto fetch = [&](int b, uint4& cw, Pair<T>& cs) {
+            if (b < limit) {
                 asm volatile("ld.global.nc.L1::no_allocate.v4.u32 {%0,%1,%2,%3}, [%4];"
                              : "=r"(cw.x), "=r"(cw.y), "=r"(cw.z), "=r"(cw.w)
-                             : "l"(my_codes + cb * 32));
-                const T* sc = my_scales + ((cb * kQ4Cols) >> a.group_log2) * kQ4Rows;
-                cs[0] = sc[0];
-                cs[1] = sc[8];
+                             : "l"(cp + b * 32));
+                cs = *reinterpret_cast<const Pair<T>*>(sp + (b >> group_shift) * kQ4Rows);
             }
         };
 #pragma unroll
-        for (int j = 0; j < kStreamAhead; ++j) fetch(j, w[j], s[j]);
+        for (int j = 0; j < kStreamAhead; ++j) fetch(wk2 + (j >> 1) * stride + (j & 1), w[j], s[j]);
 
         if (chunk != cb_begin) __syncthreads();  // the chunk before has been read
         {
@@ -340,15 +422,14 @@ __global__ void __launch_bounds__(kThreads)
         }
         __syncthreads();
 
-        for (int j0 = 0; j0 < mine; j0 += kStreamAhead) {
+        for (int b0 = wk2; b0 < limit; b0 += kStreamAhead / 2 * stride) {
 #pragma unroll
             for (int jj = 0; jj < kStreamAhead; ++jj) {
-                const int j = j0 + jj;
-                const int b = 2 * ((j >> 1) * wks + wk) + (j & 1);
+                const int b = b0 + (jj >> 1) * stride + (jj & 1);
+                if (b >= limit) continue;
                 const uint4 cw = w[jj];
-                const float s0 = to_arith<float>(s[jj][0]), s1 = to_arith<float>(s[jj][1]);
-                fetch(j + kStreamAhead, w[jj], s[jj]);
-                if (j >= mine || b >= blocks) continue;
+                const float s0 = to_arith<float>(s[jj].first), s1 = to_arith<float>(s[jj].second);
+                fetch(b + kStreamAhead / 2 * stride, w[jj], s[jj]);
                 const uint32_t word[4] = {cw.x, cw.y, cw.z, cw.w};
                 uint32_t frag[4][4];
 #pragma unroll
@@ -456,7 +537,7 @@ int q4_dequantize(const void* codes, const T* scales, T* M, int64_t nf, int64_t 
     const int64_t nrb = q4_row_blocks(nt), ncb = q4_col_blocks(nf), ng = q4_groups(nf, group);
     const int64_t total = ntasks * nrb * ncb;
     q4_dequantize_kernel<T><<<warp_grid(total), kThreads, 0, stream>>>(
-        static_cast<const uint4*>(codes), scales, M, nf, nt, nrb, ncb, ng, group, total, whole_vectors(M, nf));
+        static_cast<const uint4*>(codes), scales, M, nf, nt, nrb, ncb, ng, group == 64 ? 6 : 7, total, whole_vectors(M, nf));
     count_launch();
     return launch_status();
 }
