@@ -183,23 +183,22 @@ struct Split16<float> {
 template <typename H>
 __device__ __forceinline__ void code_pairs(uint32_t w, uint32_t (&r)[4]) {
     if constexpr (std::is_same_v<H, __half>) {
-        const __half2 off = __float2half2_rn(-1032.0f), sixteenth = __float2half2_rn(0.0625f),
-                      off16 = __float2half2_rn(-72.0f);
-#pragma unroll
-        for (int i = 0; i < 2; ++i) {
-            uint32_t lo = ((w >> (8 * i)) & 0x000f000fu) | 0x64006400u, hi = ((w >> (8 * i)) & 0x00f000f0u) | 0x64006400u;
-            const __half2 a = __hadd2(*reinterpret_cast<__half2*>(&lo), off);
-            const __half2 b = __hfma2(*reinterpret_cast<__half2*>(&hi), sixteenth, off16);
-            r[2 * i] = *reinterpret_cast<const uint32_t*>(&a);
-            r[2 * i + 1] = *reinterpret_cast<const uint32_t*>(&b);
-        }
+        const uint32_t w8 = w >> 8;
+        uint32_t t;
+        asm("lop3.b32 %0, %1, 0x000f000f, 0x64006400, 0xea;" : "=r"(t) : "r"(w));
+        asm("add.rn.f16x2 %0, %1, %2;" : "=r"(r[0]) : "r"(t), "r"(0xe408e408u));  // -1032
+        asm("lop3.b32 %0, %1, 0x00f000f0, 0x64006400, 0xea;" : "=r"(t) : "r"(w));
+        asm("fma.rn.f16x2 %0, %1, %2, %3;" : "=r"(r[1]) : "r"(t), "r"(0x2c002c00u), "r"(0xd480d480u));  // /16 - 72
+        asm("lop3.b32 %0, %1, 0x000f000f, 0x64006400, 0xea;" : "=r"(t) : "r"(w8));
+        asm("add.rn.f16x2 %0, %1, %2;" : "=r"(r[2]) : "r"(t), "r"(0xe408e408u));
+        asm("lop3.b32 %0, %1, 0x00f000f0, 0x64006400, 0xea;" : "=r"(t) : "r"(w8));
+        asm("fma.rn.f16x2 %0, %1, %2, %3;" : "=r"(r[3]) : "r"(t), "r"(0x2c002c00u), "r"(0xd480d480u));
     } else {
-        const __nv_bfloat162 off = __float2bfloat162_rn(-136.0f);
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
-            uint32_t v = ((w >> (4 * i)) & 0x000f000fu) | 0x43004300u;
-            const __nv_bfloat162 a = __hadd2(*reinterpret_cast<__nv_bfloat162*>(&v), off);
-            r[i] = *reinterpret_cast<const uint32_t*>(&a);
+            uint32_t t;
+            asm("lop3.b32 %0, %1, 0x000f000f, 0x43004300, 0xea;" : "=r"(t) : "r"(w >> (4 * i)));
+            asm("add.rn.bf16x2 %0, %1, %2;" : "=r"(r[i]) : "r"(t), "r"(0xc308c308u));  // -136
         }
     }
 }
@@ -278,7 +277,7 @@ __global__ void __launch_bounds__(kThreads)
 
 // ---- a few observations: the stream of the codes ------------------------------
 //
-// Bound by HBM: half a byte a weight, so with 1 to 32 observations the codes
+// Bound by HBM: half a byte a weight, so with 1 to 8 observations the codes
 // are nearly all that moves.  A warp takes a block of 16 targets x 64 features
 // per step: one 16-byte load per lane is the block's four tensor-core
 // fragments (mma.m16n8k16, weights as the 16-row operand), made into whole
@@ -288,15 +287,20 @@ __global__ void __launch_bounds__(kThreads)
 // observations are three bfloat16 terms (8 bits each, together all 24), each
 // with its own products.
 //
-// A CTA holds its observations' features in shared memory (in the order of
-// memory: lane 4g + c reads features 16c.. of observation g, which is what the
-// codes' order was chosen for); its eight warps share out row blocks and, where
-// a model has fewer than eight, features.  The features may also be shared by
-// the CTAs of a cluster, whose partial sums meet in distributed shared memory
-// in a fixed order.
+// One CTA to an SM, with 1/148 of a model's row blocks each (to the nearest
+// whole one) and its observations' features and scales in shared memory; the
+// row blocks' codes, laid end to end, are cut into equal runs for its warps,
+// so that no warp is left without work whatever the sizes.  A warp's sums for
+// a row block go to a slot of its own, and a row block's slots are added up
+// in the order of the warps.  Models with fewer row blocks than SMs share the
+// features out over the CTAs of a cluster as well.
 
-constexpr int kStreamChunk = 1024;  // features staged together
-constexpr int kStreamAhead = 4;     // blocks of codes in flight per warp
+constexpr int kStreamWarps = 16, kStreamThreads = kStreamWarps * 32;
+constexpr int kStreamObs = 8;     // columns of a fragment
+constexpr int kStreamAhead = 4;   // pairs of blocks (128 features) in flight per warp
+constexpr int kStreamRows = 16;   // row blocks a CTA works on together
+constexpr int kSlots = kStreamRows / kStreamWarps + 3;  // row blocks one warp's run can touch
+constexpr int kSlotLd = kQ4Rows + 1, kSlotFloats = kStreamObs * kSlotLd;
 
 template <typename H>
 __device__ __forceinline__ void mma_16816(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
@@ -334,182 +338,261 @@ struct alignas(2 * sizeof(T)) Pair {
 
 struct StreamArgs {
     int64_t nf, nt, ntasks, nobs;
-    int64_t nrb, ncb, ngroups;
-    int64_t row_groups;   // CTAs (clusters) a task's row blocks take
-    int64_t per_rank;     // 64-feature blocks to a CTA of the cluster (even)
-    int group_log2;
-    int ranks;            // CTAs of a cluster, each with its share of the features
-    int rows_log2;        // log2 of the row blocks a CTA takes; 8 >> rows_log2 warps share each one's features
+    int64_t task0;      // of blockIdx.y == 0
+    int nrb, ncb, ngroups;
+    int rows;           // row blocks of a CTA
+    int per_rank;       // 64-feature blocks to a CTA of the cluster (even)
+    int chunk;          // blocks whose features are staged together (even)
+    int group_shift;    // log2 of the blocks a group takes
+    int ranks_log2;     // CTAs of a cluster, each with its share of the features
     bool vec;
 };
 
-template <typename T, int NT>
-__global__ void __launch_bounds__(kThreads)
+// Where things lie in shared memory: features [term][obs], scales [row block][group], sums [warp][slot].
+template <typename T>
+struct StreamLayout {
+    static constexpr int kTerms = Split16<T>::kTerms;
+    int row_bytes, scales_ld;   // of one observation's features; scales of one row block (at most)
+    int scales_at, slots_at, bytes;
+    // 16 past a multiple of 128: the rows that eight lanes read together meet no bank twice
+    __host__ __device__ StreamLayout(int chunk, int obs, int rows, int group_shift)
+        : row_bytes(chunk * (kQ4Cols * 2) + 16), scales_ld((chunk >> group_shift) * kQ4Rows) {
+        scales_at = kTerms * obs * row_bytes;
+        slots_at = (scales_at + rows * scales_ld * int(sizeof(T)) + 15) / 16 * 16;
+        bytes = slots_at + kStreamWarps * kSlots * kSlotFloats * 4;
+    }
+};
+
+// GROUPS: groups in 128 features.  FLAT: the CTA takes all of its row blocks' features at once, so that the
+// codes of its row blocks lie end to end.
+template <typename T, int GROUPS, bool FLAT>
+__global__ void __launch_bounds__(kStreamThreads, 1)
     q4_stream_kernel(const T* __restrict__ X, const uint4* __restrict__ codes, const T* __restrict__ scales,
-                     T* __restrict__ Yhat, const StreamArgs a) {
+                     T* __restrict__ Yhat, StreamArgs a) {
     using H = typename Split16<T>::Type;
     constexpr int kTerms = Split16<T>::kTerms;
-    constexpr int kObs = 8 * NT;
-    constexpr int kRowBytes = kStreamChunk * 2 + 16;  // 16 past a multiple of 128: eight lanes' reads meet no bank twice
     extern __shared__ __align__(16) unsigned char smem_raw[];
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, c = lane & 3;
-    const uint32_t rank = cluster_rank();
-    const int ranks = a.ranks;  // CTAs of a cluster
-    const int64_t unit = blockIdx.x / unsigned(ranks);
-    const int64_t rg = unit % a.row_groups, task = unit / a.row_groups % a.ntasks;
-    const int64_t obs0 = unit / a.row_groups / a.ntasks * kObs;
-    const int obs_here = int(min(int64_t(kObs), a.nobs - obs0));
-    const int rows = 1 << a.rows_log2, wk = warp >> a.rows_log2, wks = kWarps >> a.rows_log2;
-    const int64_t rb = rg * rows + (warp & (rows - 1));
-    const bool live = rb < a.nrb;
-    const int64_t cb_begin = int64_t(rank) * a.per_rank, cb_end = min(a.ncb, cb_begin + a.per_rank);
-    const uint4* my_codes = codes + ((task * a.nrb + (live ? rb : 0)) * a.ncb) * 32 + lane;
-    const T* my_scales = scales + (task * a.nrb + (live ? rb : 0)) * a.ngroups * kQ4Rows + 2 * g;
-    const int group_shift = a.group_log2 - 6;
+    const int rank = int(blockIdx.x) & ((1 << a.ranks_log2) - 1), ranks = 1 << a.ranks_log2;
+    const int64_t task = a.task0 + blockIdx.y, obs0 = int64_t(blockIdx.z) * kStreamObs;
+    const int obs_here = int(min(int64_t(kStreamObs), a.nobs - obs0));
+    const int rb_begin = (int(blockIdx.x) >> a.ranks_log2) * a.rows, rb_end = min(a.nrb, rb_begin + a.rows);
+    const int cb_begin = rank * a.per_rank, cb_end = min(a.ncb, cb_begin + a.per_rank);
+    const StreamLayout<T> at(a.chunk, obs_here, min(a.rows, kStreamRows), a.group_shift);
+    T* const sm_scales = reinterpret_cast<T*>(smem_raw + at.scales_at);
+    float* const slots = reinterpret_cast<float*>(smem_raw + at.slots_at);
 
-    float total[NT][4] = {};
-    for (int64_t chunk = cb_begin; chunk < cb_end; chunk += kStreamChunk / kQ4Cols) {
-        const int blocks = int(min(int64_t(kStreamChunk / kQ4Cols), cb_end - chunk));
-        // (blocks come in pairs of 128 features: a warp's j-th is block wk2 + (j/2) * stride + j%2)
-        const int wk2 = 2 * wk, stride = 2 * wks;
-        const uint4* cp = my_codes + chunk * 32;
-        const T* sp = my_scales + ((chunk * kQ4Cols) >> a.group_log2) * kQ4Rows;
-        const int limit = live ? blocks : 0;
-        uint4 w[kStreamAhead];
-        Pair<T> s[kStreamAhead];
-        auto fetch = [&](int b, uint4& cw, Pair<T>& cs) {
-            if (b < limit) {
-                asm volatile("ld.global.nc.L1::no_allocate.v4.u32 {%0,%1,%2,%3}, [%4];"
-                             : "=r"(cw.x), "=r"(cw.y), "=r"(cw.z), "=r"(cw.w)
-                             : "l"(cp + b * 32));
-                cs = *reinterpret_cast<const Pair<T>*>(sp + (b >> group_shift) * kQ4Rows);
+    for (int rb0 = rb_begin; rb0 < rb_end; rb0 += kStreamRows) {
+        const int rows = min(kStreamRows, rb_end - rb0);
+        // the first row block this warp's runs can touch, whatever the chunk's length
+        const int first_row = max(0, warp * rows / kStreamWarps - 1);
+        float* const my_slots = slots + warp * kSlots * kSlotFloats;
+        for (int i = lane; i < kSlots * kSlotFloats; i += 32) my_slots[i] = 0.0f;
+        for (int chunk = cb_begin; chunk < cb_end; chunk += a.chunk) {
+            const int blocks = min(a.chunk, cb_end - chunk);
+            // this warp's run of the row blocks' codes laid end to end, in pairs of blocks
+            const int pairs = blocks / 2;
+            const int run0 = rows * pairs * warp / kStreamWarps, run1 = rows * pairs * (warp + 1) / kStreamWarps;
+            int row = run0 / pairs, left_in_row = pairs - (run0 - row * pairs);
+            const int col0 = pairs - left_in_row;
+            const uint4* ahead = codes + ((task * a.nrb + rb0 + row) * a.ncb + chunk + 2 * col0) * 32 + lane;
+            int ahead_left = run1 - run0, ahead_in_row = left_in_row;
+            const int64_t skip = int64_t(a.ncb - blocks) * 32;
+            uint4 w[kStreamAhead][2];
+            auto fetch = [&](uint4 (&cw)[2]) {
+                if (ahead_left > 0) {
+                    asm volatile("ld.global.nc.L1::no_allocate.v4.u32 {%0,%1,%2,%3}, [%4];"
+                                 : "=r"(cw[0].x), "=r"(cw[0].y), "=r"(cw[0].z), "=r"(cw[0].w)
+                                 : "l"(ahead));
+                    asm volatile("ld.global.nc.L1::no_allocate.v4.u32 {%0,%1,%2,%3}, [%4];"
+                                 : "=r"(cw[1].x), "=r"(cw[1].y), "=r"(cw[1].z), "=r"(cw[1].w)
+                                 : "l"(ahead + 32));
+                }
+                --ahead_left;
+                ahead += 64;
+                if (!FLAT && --ahead_in_row == 0) {
+                    ahead_in_row = pairs;
+                    ahead += skip;
+                }
+            };
+#pragma unroll
+            for (int j = 0; j < kStreamAhead; ++j) fetch(w[j]);
+
+            if (chunk != cb_begin || rb0 != rb_begin) __syncthreads();  // what was staged has been read
+            const int per_row = pairs * GROUPS * kQ4Rows;  // scales of a row block, row block after row block
+            for (int i = tid; i < rows * per_row; i += kStreamThreads) {
+                const int r = i / per_row, e = i - r * per_row;
+                sm_scales[i] = scales[((task * a.nrb + rb0 + r) * a.ngroups + chunk / 2 * GROUPS) * kQ4Rows + e];
             }
-        };
+            if (rb0 == rb_begin || a.chunk < a.per_rank) {
+                constexpr int kPer = 16 / sizeof(T);
+                const int64_t f0 = int64_t(chunk) * kQ4Cols;
+                const int in = int(min(int64_t(blocks) * kQ4Cols, a.nf - f0));  // features of X; zero up to the block's end
+                const int per_obs = blocks * (kQ4Cols / kPer);
+#pragma unroll 2
+                for (int i = tid; i < obs_here * per_obs; i += kStreamThreads) {
+                    const int o = i / per_obs, f = (i - o * per_obs) * kPer;
+                    const T* src = X + ((obs0 + o) * a.ntasks + task) * a.nf + f0 + f;
+                    T v[kPer] = {};
+                    if (a.vec) {
+                        if (f < in) VecLoad<T, kPer>::load(src, v);
+                    } else {
 #pragma unroll
-        for (int j = 0; j < kStreamAhead; ++j) fetch(wk2 + (j >> 1) * stride + (j & 1), w[j], s[j]);
-
-        if (chunk != cb_begin) __syncthreads();  // the chunk before has been read
-        {
-            constexpr int kPer = 16 / sizeof(T);
-            const int64_t f0 = chunk * kQ4Cols;
-            const int feats = blocks * kQ4Cols;
-            for (int i = tid; i < obs_here * (feats / kPer); i += kThreads) {
-                const int o = i / (feats / kPer), f = i % (feats / kPer) * kPer;
-                const T* src = X + ((obs0 + o) * a.ntasks + task) * a.nf + f0 + f;
-                T v[kPer] = {};
-                if (a.vec) {
-                    if (f0 + f < a.nf) VecLoad<T, kPer>::load(src, v);
-                } else {
+                        for (int e = 0; e < kPer; ++e)
+                            if (f + e < in) v[e] = src[e];
+                    }
+                    alignas(16) H t[kTerms][kPer];
 #pragma unroll
-                    for (int e = 0; e < kPer; ++e)
-                        if (f0 + f + e < a.nf) v[e] = src[e];
-                }
-                H t[kTerms][kPer];
+                    for (int e = 0; e < kPer; ++e) {
+                        H one[kTerms];
+                        split_terms<T>(v[e], one);
 #pragma unroll
-                for (int e = 0; e < kPer; ++e) {
-                    H one[kTerms];
-                    split_terms<T>(v[e], one);
+                        for (int q = 0; q < kTerms; ++q) t[q][e] = one[q];
+                    }
 #pragma unroll
-                    for (int q = 0; q < kTerms; ++q) t[q][e] = one[q];
-                }
-#pragma unroll
-                for (int q = 0; q < kTerms; ++q) {
-                    unsigned char* dst = smem_raw + (q * kObs + o) * kRowBytes + f * 2;
-                    if constexpr (kPer == 8) *reinterpret_cast<uint4*>(dst) = *reinterpret_cast<const uint4*>(t[q]);
-                    else *reinterpret_cast<uint2*>(dst) = *reinterpret_cast<const uint2*>(t[q]);
+                    for (int q = 0; q < kTerms; ++q) {
+                        unsigned char* dst = smem_raw + (q * obs_here + o) * at.row_bytes + f * 2;
+                        if constexpr (kPer == 8) *reinterpret_cast<uint4*>(dst) = *reinterpret_cast<const uint4*>(t[q]);
+                        else *reinterpret_cast<uint2*>(dst) = *reinterpret_cast<const uint2*>(t[q]);
+                    }
                 }
             }
-        }
-        __syncthreads();
+            __syncthreads();
 
-        for (int b0 = wk2; b0 < limit; b0 += kStreamAhead / 2 * stride) {
+            // observations past the last one read another's row; their columns are not stored
+            const unsigned char* const x0 = smem_raw + min(g, obs_here - 1) * at.row_bytes + 32 * c;
+            const unsigned char* x = x0 + col0 * (kQ4Cols * 4);
+            const T* sc = sm_scales + run0 * (GROUPS * kQ4Rows) + 2 * g;
+            const int term_bytes = obs_here * at.row_bytes;
+            float total[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+            auto flush = [&] {
+                float* slot = my_slots + (row - first_row) * kSlotFloats + 2 * c * kSlotLd + g;
+                slot[0] += total[0];
+                slot[kSlotLd] += total[1];
+                slot[8] += total[2];
+                slot[kSlotLd + 8] += total[3];
+            };
+            auto add = [&](const float (&acc)[4], const T* at_scale) {
+                const Pair<T> s = *reinterpret_cast<const Pair<T>*>(at_scale);
+                const float s0 = to_arith<float>(s.first), s1 = to_arith<float>(s.second);
+                total[0] = fmaf(s0, acc[0], total[0]);
+                total[1] = fmaf(s0, acc[1], total[1]);
+                total[2] = fmaf(s1, acc[2], total[2]);
+                total[3] = fmaf(s1, acc[3], total[3]);
+            };
+            for (int left = run1 - run0; left > 0; left -= kStreamAhead) {
 #pragma unroll
-            for (int jj = 0; jj < kStreamAhead; ++jj) {
-                const int b = b0 + (jj >> 1) * stride + (jj & 1);
-                if (b >= limit) continue;
-                const uint4 cw = w[jj];
-                const float s0 = to_arith<float>(s[jj].first), s1 = to_arith<float>(s[jj].second);
-                fetch(b + kStreamAhead / 2 * stride, w[jj], s[jj]);
-                const uint32_t word[4] = {cw.x, cw.y, cw.z, cw.w};
-                uint32_t frag[4][4];
+                for (int j = 0; j < kStreamAhead; ++j) {
+                    if (j >= left) break;
+                    uint32_t frag[2][4][4];
 #pragma unroll
-                for (int k = 0; k < 4; ++k) code_pairs<H>(word[k], frag[k]);
-#pragma unroll
-                for (int n = 0; n < NT; ++n) {
-                    // observations past the last one read another's row; their columns are not stored
-                    const int o = min(8 * n + g, obs_here - 1);
+                    for (int h = 0; h < 2; ++h) {
+                        code_pairs<H>(w[j][h].x, frag[h][0]);
+                        code_pairs<H>(w[j][h].y, frag[h][1]);
+                        code_pairs<H>(w[j][h].z, frag[h][2]);
+                        code_pairs<H>(w[j][h].w, frag[h][3]);
+                    }
+                    fetch(w[j]);
                     float acc[4] = {0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
-                    for (int q = kTerms - 1; q >= 0; --q) {
-                        const uint4* x = reinterpret_cast<const uint4*>(smem_raw + (q * kObs + o) * kRowBytes +
-                                                                        (b * kQ4Cols + 16 * c) * 2);
-                        const uint4 x0 = x[0], x1 = x[1];
-                        mma_16816<H>(acc, frag[0], x0.x, x0.y);
-                        mma_16816<H>(acc, frag[1], x0.z, x0.w);
-                        mma_16816<H>(acc, frag[2], x1.x, x1.y);
-                        mma_16816<H>(acc, frag[3], x1.z, x1.w);
+                    for (int h = 0; h < 2; ++h) {
+#pragma unroll
+                        for (int q = kTerms - 1; q >= 0; --q) {
+                            const uint4* xv = reinterpret_cast<const uint4*>(x + q * term_bytes + h * (kQ4Cols * 2));
+                            const uint4 lo = xv[0], hi = xv[1];
+                            mma_16816<H>(acc, frag[h][0], lo.x, lo.y);
+                            mma_16816<H>(acc, frag[h][1], lo.z, lo.w);
+                            mma_16816<H>(acc, frag[h][2], hi.x, hi.y);
+                            mma_16816<H>(acc, frag[h][3], hi.z, hi.w);
+                        }
+                        if (GROUPS == 2) {
+                            add(acc, sc + h * kQ4Rows);
+                            acc[0] = acc[1] = acc[2] = acc[3] = 0.0f;
+                        }
                     }
-                    total[n][0] = fmaf(s0, acc[0], total[n][0]);
-                    total[n][1] = fmaf(s0, acc[1], total[n][1]);
-                    total[n][2] = fmaf(s1, acc[2], total[n][2]);
-                    total[n][3] = fmaf(s1, acc[3], total[n][3]);
+                    if (GROUPS == 1) add(acc, sc);
+                    x += kQ4Cols * 4;
+                    sc += GROUPS * kQ4Rows;
+                    if (--left_in_row == 0) {
+                        flush();
+                        total[0] = total[1] = total[2] = total[3] = 0.0f;
+                        left_in_row = pairs;
+                        x = x0;
+                        ++row;
+                    }
                 }
             }
+            if (left_in_row < pairs && run1 > run0) flush();
         }
-    }
 
-    // ---- the warps' and the cluster's partial sums ----
-    __syncthreads();
-    constexpr int kPartLd = kQ4Rows + 1;
-    float* part = reinterpret_cast<float*>(smem_raw);  // [warp][obs][16 targets]
-#pragma unroll
-    for (int n = 0; n < NT; ++n)
-#pragma unroll
-        for (int i = 0; i < 4; ++i)
-            part[(warp * kObs + 8 * n + 2 * c + (i & 1)) * kPartLd + g + 8 * (i >> 1)] = total[n][i];
-    __syncthreads();
-    if (ranks > 1) cluster_sync();
-    const int outputs = rows * kQ4Rows * obs_here;
-    const int begin = outputs * int(rank) / ranks, end = outputs * (int(rank) + 1) / ranks;
-    for (int i = begin + tid; i < end; i += kThreads) {
-        const int o = i / (rows * kQ4Rows), t = i % (rows * kQ4Rows);
-        const int64_t target = rg * rows * kQ4Rows + t;
-        float v = 0.0f;
-        for (int r = 0; r < ranks; ++r)
-            for (int k = 0; k < wks; ++k) {
-                const float* at = part + ((k * rows + t / kQ4Rows) * kObs + o) * kPartLd + t % kQ4Rows;
-                v += ranks > 1 ? ld_cluster_f32(at, r) : *at;
-            }
-        if (target < a.nt) Yhat[((obs0 + o) * a.ntasks + task) * a.nt + target] = from_arith<T>(v);
+        __syncthreads();
+        if (ranks > 1) cluster_sync();
+        const int outputs = rows * kQ4Rows;
+        for (int i = rank * kStreamThreads + tid; i < outputs * obs_here; i += ranks * kStreamThreads) {
+            const int o = i / outputs, t = i - o * outputs, r = t / kQ4Rows;
+            const int64_t target = int64_t(rb0) * kQ4Rows + t;
+            float v = 0.0f;
+            for (int p = 0; p < ranks; ++p)
+                for (int k = 0; k < kStreamWarps; ++k) {
+                    const int slot = r - max(0, k * rows / kStreamWarps - 1);
+                    if (slot < 0) break;
+                    if (slot >= kSlots) continue;
+                    const float* from = slots + (k * kSlots + slot) * kSlotFloats + o * kSlotLd + t % kQ4Rows;
+                    v += ranks > 1 ? ld_cluster_f32(from, p) : *from;
+                }
+            if (target < a.nt) Yhat[((obs0 + o) * a.ntasks + task) * a.nt + target] = from_arith<T>(v);
+        }
+        if (ranks > 1) cluster_sync_relaxed();  // the peers have read this CTA's sums
+        else if (rb0 + kStreamRows < rb_end) __syncthreads();
     }
-    if (ranks > 1) cluster_sync_relaxed();  // the peers have read this CTA's sums
 }
 
-template <typename T, int NT>
-int stream_launch(const T* X, const void* codes, const T* scales, T* Yhat, const StreamArgs& a,
-                  cudaStream_t stream) {
-    const size_t smem = std::max(size_t(Split16<T>::kTerms) * 8 * NT * (kStreamChunk * 2 + 16),
-                                 size_t(kWarps) * 8 * NT * (kQ4Rows + 1) * 4);
-    static std::atomic<uint64_t> attr{0};
-    auto kernel = q4_stream_kernel<T, NT>;
-    cudaError_t e = set_smem_limit_once(attr, kernel, smem);
+template <typename T>
+int stream_predict(const T* X, const void* codes, const T* scales, T* Yhat, StreamArgs a, cudaStream_t stream) {
+    constexpr size_t kRoom = size_t(224) * 1024;
+    const int obs = int(std::min<int64_t>(kStreamObs, a.nobs));
+    const int64_t obs_tiles = (a.nobs + kStreamObs - 1) / kStreamObs, sms = sm_count();
+    // CTAs for a task's row blocks, one to an SM
+    const int64_t ctas = std::max<int64_t>(1, sms / std::min(sms, a.ntasks * obs_tiles));
+    a.rows = int((a.nrb + ctas - 1) / ctas);
+    const int64_t groups = (a.nrb + a.rows - 1) / a.rows;
+    // CTAs of a cluster: while they find SMs and each warp two blocks of codes
+    while (a.ranks_log2 < 3 && ((groups * a.ntasks * obs_tiles) << (a.ranks_log2 + 1)) <= sms &&
+           int64_t(a.ncb) * a.rows >= (2 * kStreamWarps) << (a.ranks_log2 + 1))
+        ++a.ranks_log2;
+    const int ranks = 1 << a.ranks_log2, rows = std::min(a.rows, kStreamRows);
+    a.per_rank = ((a.ncb + ranks - 1) / ranks + 1) / 2 * 2;
+    // the longest run of features that leaves room for the scales and sums
+    a.chunk = a.per_rank;
+    while (size_t(StreamLayout<T>(a.chunk, obs, rows, a.group_shift).bytes) > kRoom) a.chunk = (a.chunk / 2 + 1) / 2 * 2;
+    const bool flat = a.chunk >= a.ncb;
+    static std::atomic<uint64_t> attr[4];
+    void (*const kernels[4])(const T*, const uint4*, const T*, T*, StreamArgs) = {
+        q4_stream_kernel<T, 1, false>, q4_stream_kernel<T, 1, true>, q4_stream_kernel<T, 2, false>,
+        q4_stream_kernel<T, 2, true>};
+    const int which = (a.group_shift == 0 ? 2 : 0) + (flat ? 1 : 0);
+    const auto kernel = kernels[which];
+    cudaError_t e = set_smem_limit_once(attr[which], kernel, kRoom);
     if (e != cudaSuccess) return int(e);
+    if (obs_tiles > 65535 || (groups << a.ranks_log2) > 0x7fffffff) return GLMB_ERR_TOO_LARGE;
     cudaLaunchConfig_t cfg = {};
-    const int64_t units = a.row_groups * a.ntasks * ((a.nobs + 8 * NT - 1) / (8 * NT));
-    if (units > (int64_t(1) << 31) / a.ranks - 1) return GLMB_ERR_TOO_LARGE;
-    cfg.gridDim = dim3(unsigned(units * a.ranks));
-    cfg.blockDim = dim3(kThreads);
-    cfg.dynamicSmemBytes = smem;
+    cfg.blockDim = dim3(kStreamThreads);
+    cfg.dynamicSmemBytes = size_t(StreamLayout<T>(a.chunk, obs, rows, a.group_shift).bytes);
     cfg.stream = stream;
     cudaLaunchAttribute at[1];
     at[0].id = cudaLaunchAttributeClusterDimension;
-    at[0].val.clusterDim.x = unsigned(a.ranks);
+    at[0].val.clusterDim.x = unsigned(ranks);
     at[0].val.clusterDim.y = at[0].val.clusterDim.z = 1;
     cfg.attrs = at;
     cfg.numAttrs = 1;
-    count_launch();
-    e = cudaLaunchKernelEx(&cfg, kernel, X, static_cast<const uint4*>(codes), scales, Yhat, a);
-    return e != cudaSuccess ? int(e) : launch_status();
+    for (a.task0 = 0; a.task0 < a.ntasks; a.task0 += 65535) {
+        cfg.gridDim = dim3(unsigned(groups << a.ranks_log2), unsigned(std::min<int64_t>(65535, a.ntasks - a.task0)),
+                           unsigned(obs_tiles));
+        count_launch();
+        e = cudaLaunchKernelEx(&cfg, kernel, X, static_cast<const uint4*>(codes), scales, Yhat, StreamArgs(a));
+        if (e != cudaSuccess) return int(e);
+    }
+    return launch_status();
 }
 
 template <typename T>
@@ -551,19 +634,11 @@ template <typename T>
 int q4_predict(const T* X, const void* codes, const T* scales, T* Yhat, int64_t nf, int64_t nt, int64_t ntasks,
                int64_t nobs, int group, void*, size_t, cudaStream_t stream) {
     const int64_t nrb = q4_row_blocks(nt), ncb = q4_col_blocks(nf), ng = q4_groups(nf, group);
-    StreamArgs a{nf, nt, ntasks, nobs, nrb, ncb, ng, 0, 0, group == 64 ? 6 : 7, 1, 0, whole_vectors(X, nf)};
-    while (a.rows_log2 < 3 && (int64_t(1) << a.rows_log2) < nrb) ++a.rows_log2;
-    a.row_groups = (nrb + (int64_t(1) << a.rows_log2) - 1) >> a.rows_log2;
-    // CTAs that share a row group's features: until every SM has four CTAs, while each keeps 128 features a warp
-    const int64_t least = 2 * (kWarps >> a.rows_log2);
-    while (a.ranks < 8 && a.row_groups * ntasks * a.ranks * 2 <= 4 * int64_t(sm_count()) &&
-           ncb >= 2 * a.ranks * least)
-        a.ranks *= 2;
-    a.per_rank = ((ncb + a.ranks - 1) / a.ranks + 1) / 2 * 2;
+    if (nrb > (1 << 30) || ncb > (1 << 20)) return GLMB_ERR_TOO_LARGE;
+    StreamArgs a{nf, nt, ntasks, nobs, 0, int(nrb), int(ncb), int(ng), 0, 0, 0, group == 64 ? 0 : 1, 0,
+                 whole_vectors(X, nf)};
     set_last_path("q4_stream");
-    if (nobs <= 8) return stream_launch<T, 1>(X, codes, scales, Yhat, a, stream);
-    if (nobs <= 16) return stream_launch<T, 2>(X, codes, scales, Yhat, a, stream);
-    return stream_launch<T, 4>(X, codes, scales, Yhat, a, stream);
+    return stream_predict<T>(X, codes, scales, Yhat, a, stream);
 }
 
 #define GLMB_INSTANTIATE_Q4(T)                                                                                \

@@ -10,8 +10,9 @@ constexpr int kQ4Cols = 64;   // features of a block of codes
 constexpr int kQ4BlockBytes = kQ4Rows * kQ4Cols / 2;
 
 inline int64_t q4_row_blocks(int64_t nt) { return (nt + kQ4Rows - 1) / kQ4Rows; }
-inline int64_t q4_col_blocks(int64_t nf) { return (nf + kQ4Cols - 1) / kQ4Cols; }
-inline int64_t q4_groups(int64_t nf, int group) { return (nf + group - 1) / group; }
+// features are filled up to a multiple of 128, whole groups of either size
+inline int64_t q4_col_blocks(int64_t nf) { return (nf + 2 * kQ4Cols - 1) / (2 * kQ4Cols) * 2; }
+inline int64_t q4_groups(int64_t nf, int group) { return q4_col_blocks(nf) * kQ4Cols / group; }
 
 template <typename T>
 int q4_quantize(const T* M, void* codes, T* scales, int64_t nf, int64_t nt, int64_t ntasks, int group,

@@ -87,7 +87,8 @@ GLMM_DECLARE_ORTHO(bf16, uint16_t)
  *          four bits; from bit 0 up: (g, f), (g+8, f), (g, f+2), (g+8, f+2),
  *          and from bit 16 up the same of f + 1 and f + 3;
  *   scales [task][target/16][group][target%8][target/8%2].
- * Targets and features that fill up the last block have code 0.
+ * Targets are filled up to a multiple of 16 and features to one of 128; what
+ * fills up has code 0, and groups of nothing else s = 0.
  * ---------------------------------------------------------------------- */
 int64_t glmm_q4_codes_bytes(int64_t nfeatures, int64_t ntargets, int64_t ntasks);
 int64_t glmm_q4_scales_count(int64_t nfeatures, int64_t ntargets, int64_t ntasks, int group);

@@ -99,11 +99,12 @@ def test_q4_refusals(sfx):
 
 def test_q4_sizes():
     L = capi.lib()
-    # 16 x 64 blocks of 512 bytes; scales padded to 16 targets
+    # 16 x 64 blocks of 512 bytes; scales padded to 16 targets; features to a multiple of 128
     assert L.glmm_q4_codes_bytes(256, 16, 64) == 64 * 4 * 512
     assert L.glmm_q4_codes_bytes(65, 17, 1) == 2 * 2 * 512
     assert L.glmm_q4_scales_count(65, 17, 3, 64) == 3 * 32 * 2
     assert L.glmm_q4_scales_count(129, 1, 1, 128) == 16 * 2
+    assert L.glmm_q4_codes_bytes(8, 4, 1) == 2 * 512 and L.glmm_q4_scales_count(8, 4, 1, 64) == 16 * 2
     assert L.glmm_q4_codes_bytes(0, 4, 1) == 0 and L.glmm_q4_codes_bytes(-1, 4, 1) == 0
     assert L.glmm_q4_scales_count(64, 4, 1, 32) == 0
 
@@ -126,7 +127,7 @@ def test_wrappers_refuse_before_any_launch():
     with pytest.raises(ValueError, match="group"):
         glm.Q4Model((1, 4, 8), torch.float32, 32, "cpu")
     model = glm.Q4Model((1, 4, 8), torch.float32, 64, "cpu")
-    assert model.codes.numel() == 512 and model.scales.numel() == 16 and model.device.type == "cpu"
+    assert model.codes.numel() == 1024 and model.scales.numel() == 32 and model.device.type == "cpu"
     with pytest.raises(ValueError, match="CUDA"):
         glm.predict_q4(torch.zeros(2, 1, 8), model)
     assert capi.launch_count() == before
