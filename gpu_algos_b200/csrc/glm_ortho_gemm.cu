@@ -306,6 +306,9 @@ __global__ void __launch_bounds__(kThreads, 1)
                     commit<PAIR>(&sm.accf[buf], mask);
                 }
                 commit<PAIR>(&sm.done, mask);
+                // no CTA leaves while a draining warp's arrival is on its way to it
+                for (int b = 0; b < 2 && b < nkb; ++b)
+                    mbar_wait(&sm.acce[b], uint32_t(((nkb - b + 1) / 2 - 1) & 1), failed);
             }
             mbar_wait(&sm.done, 0, nullptr);
         } else if (PAIR && warp == 2 && lane == 0 && rank != lead) {

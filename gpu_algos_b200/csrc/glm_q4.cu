@@ -7,7 +7,7 @@
 // written out in glm_matrix_b200.h).
 #include <algorithm>
 
-#include "glm_q4.cuh"
+#include "glm_q4_device.cuh"
 #include "glm_tc.cuh"
 
 namespace glmb {
@@ -165,44 +165,6 @@ __global__ void __launch_bounds__(kThreads)
     }
 }
 
-// The 16-bit type the tensor core multiplies in, and how many terms an X takes.
-template <typename T>
-struct Split16 {
-    using Type = T;
-    static constexpr int kTerms = 1;
-};
-template <>
-struct Split16<float> {
-    using Type = __nv_bfloat16;
-    static constexpr int kTerms = 3;
-};
-
-// The four pairs of a word of codes (u = q + 8) as 16-bit floats q: the code is put under the leading bit of
-// a power of two (1024 + u or, four bits up, 1024 + 16u in binary16; 128 + u in bfloat16) and the offset taken
-// off again, exactly.
-template <typename H>
-__device__ __forceinline__ void code_pairs(uint32_t w, uint32_t (&r)[4]) {
-    if constexpr (std::is_same_v<H, __half>) {
-        const uint32_t w8 = w >> 8;
-        uint32_t t;
-        asm("lop3.b32 %0, %1, 0x000f000f, 0x64006400, 0xea;" : "=r"(t) : "r"(w));
-        asm("add.rn.f16x2 %0, %1, %2;" : "=r"(r[0]) : "r"(t), "r"(0xe408e408u));  // -1032
-        asm("lop3.b32 %0, %1, 0x00f000f0, 0x64006400, 0xea;" : "=r"(t) : "r"(w));
-        asm("fma.rn.f16x2 %0, %1, %2, %3;" : "=r"(r[1]) : "r"(t), "r"(0x2c002c00u), "r"(0xd480d480u));  // /16 - 72
-        asm("lop3.b32 %0, %1, 0x000f000f, 0x64006400, 0xea;" : "=r"(t) : "r"(w8));
-        asm("add.rn.f16x2 %0, %1, %2;" : "=r"(r[2]) : "r"(t), "r"(0xe408e408u));
-        asm("lop3.b32 %0, %1, 0x00f000f0, 0x64006400, 0xea;" : "=r"(t) : "r"(w8));
-        asm("fma.rn.f16x2 %0, %1, %2, %3;" : "=r"(r[3]) : "r"(t), "r"(0x2c002c00u), "r"(0xd480d480u));
-    } else {
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-            uint32_t t;
-            asm("lop3.b32 %0, %1, 0x000f000f, 0x43004300, 0xea;" : "=r"(t) : "r"(w >> (4 * i)));
-            asm("add.rn.bf16x2 %0, %1, %2;" : "=r"(r[i]) : "r"(t), "r"(0xc308c308u));  // -136
-        }
-    }
-}
-
 // A pair of codes times a scale, rounded to T, as the 32-bit words of two elements of T (one for 16-bit types).
 template <typename T>
 __device__ __forceinline__ void scaled_pair(uint32_t pair, T s, uint32_t* dst) {
@@ -315,26 +277,6 @@ __device__ __forceinline__ void mma_16816(float (&d)[4], const uint32_t (&a)[4],
             : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
             : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
 }
-
-// x as a sum of terms of the tensor core's type (one for a 16-bit x, three for a float)
-template <typename T>
-__device__ __forceinline__ void split_terms(T x, typename Split16<T>::Type (&t)[Split16<T>::kTerms]) {
-    if constexpr (std::is_same_v<T, float>) {
-        // a NaN or an infinity stays in the first term alone
-        t[0] = __float2bfloat16_rn(x);
-        const float r1 = x - __bfloat162float(t[0]);
-        const bool finite = fabsf(__bfloat162float(t[0])) <= 3.402823466e38f;
-        t[1] = __float2bfloat16_rn(finite ? r1 : 0.0f);
-        t[2] = __float2bfloat16_rn(finite ? r1 - __bfloat162float(t[1]) : 0.0f);
-    } else {
-        t[0] = x;
-    }
-}
-
-template <typename T>
-struct alignas(2 * sizeof(T)) Pair {
-    T first, second;
-};
 
 struct StreamArgs {
     int64_t nf, nt, ntasks, nobs;
@@ -625,16 +567,24 @@ int q4_dequantize(const void* codes, const T* scales, T* M, int64_t nf, int64_t 
     return launch_status();
 }
 
+// Up to this many observations go through the stream kernel (one pass over the codes per eight of them).
+constexpr int64_t kStreamMost = 8;
+
 template <typename T>
-size_t q4_predict_workspace(int64_t, int64_t, int64_t, int64_t, int) {
-    return 0;
+size_t q4_predict_workspace(int64_t nf, int64_t nt, int64_t ntasks, int64_t nobs, int group) {
+    return nobs <= kStreamMost ? 0 : q4_tile_workspace<T>(nf, ntasks, nobs);
 }
 
 template <typename T>
 int q4_predict(const T* X, const void* codes, const T* scales, T* Yhat, int64_t nf, int64_t nt, int64_t ntasks,
-               int64_t nobs, int group, void*, size_t, cudaStream_t stream) {
+               int64_t nobs, int group, void* ws, size_t ws_bytes, cudaStream_t stream) {
     const int64_t nrb = q4_row_blocks(nt), ncb = q4_col_blocks(nf), ng = q4_groups(nf, group);
-    if (nrb > (1 << 30) || ncb > (1 << 20)) return GLMB_ERR_TOO_LARGE;
+    if (nrb > (1 << 27) || ncb > (1 << 20)) return GLMB_ERR_TOO_LARGE;
+    if (nobs > kStreamMost) {
+        set_last_path("q4_tile");
+        return q4_tile_predict<T>(X, codes, scales, Yhat, nf, nt, ntasks, nobs, group, whole_vectors(X, nf), ws,
+                                  ws_bytes, stream);
+    }
     StreamArgs a{nf, nt, ntasks, nobs, 0, int(nrb), int(ncb), int(ng), 0, 0, 0, group == 64 ? 0 : 1, 0,
                  whole_vectors(X, nf)};
     set_last_path("q4_stream");

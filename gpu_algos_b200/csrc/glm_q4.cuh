@@ -26,4 +26,11 @@ template <typename T>
 int q4_predict(const T* X, const void* codes, const T* scales, T* Yhat, int64_t nf, int64_t nt, int64_t ntasks,
                int64_t nobs, int group, void* ws, size_t ws_bytes, cudaStream_t stream);
 
+// Many observations: glm_q4_tile.cu.  `vec`: X's rows are whole 16-byte pieces.
+template <typename T>
+size_t q4_tile_workspace(int64_t nf, int64_t ntasks, int64_t nobs);
+template <typename T>
+int q4_tile_predict(const T* X, const void* codes, const T* scales, T* Yhat, int64_t nf, int64_t nt, int64_t ntasks,
+                    int64_t nobs, int group, bool vec, void* ws, size_t ws_bytes, cudaStream_t stream);
+
 }  // namespace glmb
