@@ -27,12 +27,12 @@ namespace glmb {
 namespace {
 
 constexpr int kBM = 128;  // targets per CTA
-constexpr int kBK = 64;   // features per stage: one 128-byte swizzle row, one block of codes
+constexpr int kBK = 64;   // features of a block of codes: one 128-byte swizzle row
 constexpr int kATileBytes = kBM * kBK * 2;
 constexpr int kDrainWarp0 = 4, kDrainWarps = 8;
 constexpr int kMakeWarp0 = kDrainWarp0 + kDrainWarps, kMakeWarps = 8;  // a row block of the tile each
 constexpr int kThreads = (kMakeWarp0 + kMakeWarps) * 32;
-constexpr int kMakeAhead = 4;  // blocks of codes in flight per warp
+constexpr int kMakeAhead = 4;  // blocks of codes in flight per warp (whole stages)
 constexpr int kMaxSplits = 4;
 // 640 threads launch with 96 registers each; control and making warps give to those that drain
 constexpr uint32_t kRegsControl = 40, kRegsDrain = 168, kRegsMake = 48;
@@ -41,9 +41,12 @@ static_assert(128 * kRegsControl + 256 * kRegsDrain + 256 * kRegsMake <= kThread
 template <typename T, int N>
 struct TileShape {
     static constexpr int kTerms = Split16<T>::kTerms;
+    // blocks per stage: two, so that handing a stage over (a proxy fence and an arrival, by every warp that
+    // makes operands) is paid half as often; the three terms of a float X leave room for one
+    static constexpr int kSub = kTerms == 1 ? 2 : 1;
     static constexpr int kXTermBytes = N / 2 * kBK * 2;  // this CTA's observations, one term
     static constexpr int kXBytes = kTerms * kXTermBytes;
-    static constexpr int kStageBytes = kATileBytes + kXBytes;
+    static constexpr int kStageBytes = kSub * (kATileBytes + kXBytes);  // operands, then X, block by block
     static constexpr int kStages = std::min(8, 192 * 1024 / kStageBytes);
     static constexpr int kCols = N / 2;  // observations a draining thread sums
 };
@@ -106,7 +109,7 @@ __global__ void __launch_bounds__(kThreads, 1)
                    const T* __restrict__ scales, T* __restrict__ Yhat, const TileArgs a) {
     using S = TileShape<T, N>;
     using H = typename Split16<T>::Type;
-    constexpr int kStages = S::kStages, kCols = S::kCols;
+    constexpr int kStages = S::kStages, kCols = S::kCols, kSub = S::kSub;
     constexpr uint32_t kTmemCols = N < 32 ? 32 : 2 * N;
     extern __shared__ __align__(1024) unsigned char smem_raw[];
     TileSmem<T, N>& sm = *reinterpret_cast<TileSmem<T, N>*>(
@@ -124,6 +127,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     const int kb0 = int(int64_t(a.ncb / 2) * part / a.splits) * 2, kb1 = int(int64_t(a.ncb / 2) * (part + 1) / a.splits) * 2;
     const int nkb = kb1 - kb0;
     const int gb = 1 << a.group_shift;  // blocks accumulated together
+    const int nst = nkb / kSub;
 
     if (tid == 0) {
         asm volatile("prefetch.tensormap [%0];" ::"l"(&map_x) : "memory");
@@ -159,38 +163,48 @@ __global__ void __launch_bounds__(kThreads, 1)
         if (warp == 0 && lane == 0) {
             pdl_wait_for_producer();  // X may be the terms that the kernel before wrote
             int issued = 0;
-            for (int kb = 0; kb < nkb; ++kb) {
-                const int s = kb % kStages;
-                if (kb >= kStages && !mbar_wait(&sm.empty[s], uint32_t((kb / kStages - 1) & 1), failed)) break;
-                mbar_expect_tx(&sm.xfull[s], S::kXBytes);
-                tma_load_4d(sm.stage[s] + kATileBytes, &map_x, (kb0 + kb) * kBK, int(n0 + half * (N / 2)), int(task), 0,
-                            &sm.xfull[s]);
-                issued = kb + 1;
+            for (int st = 0; st < nst; ++st) {
+                const int s = st % kStages;
+                if (st >= kStages && !mbar_wait(&sm.empty[s], uint32_t((st / kStages - 1) & 1), failed)) break;
+                mbar_expect_tx(&sm.xfull[s], kSub * S::kXBytes);
+#pragma unroll
+                for (int j = 0; j < kSub; ++j)
+                    tma_load_4d(sm.stage[s] + kSub * kATileBytes + j * S::kXBytes, &map_x, (kb0 + st * kSub + j) * kBK,
+                                int(n0 + half * (N / 2)), int(task), 0, &sm.xfull[s]);
+                issued = st + 1;
             }
             // the copies still in flight land before shared memory is used for anything else
-            for (int kb = issued > kStages ? issued - kStages : 0; kb < issued; ++kb)
-                mbar_wait(&sm.xfull[kb % kStages], uint32_t((kb / kStages) & 1), nullptr);
+            for (int st = issued > kStages ? issued - kStages : 0; st < issued; ++st)
+                mbar_wait(&sm.xfull[st % kStages], uint32_t((st / kStages) & 1), nullptr);
         } else if (warp == 1 && lane == 0) {
             if (rank == lead) {
                 constexpr uint32_t idesc = instr_desc_16<H>(256, N);
                 const uint16_t mask = uint16_t(3u << lead);
-                for (int kb = 0; kb < nkb; ++kb) {
-                    const int s = kb % kStages, grp = kb >> a.group_shift, buf = grp & 1;
-                    const bool first = (kb & (gb - 1)) == 0;
-                    if (first && grp >= 2 && !mbar_wait(&sm.acce[buf], uint32_t(((grp >> 1) - 1) & 1), failed)) break;
-                    if (!mbar_wait(&sm.ready[s], uint32_t((kb / kStages) & 1), failed)) break;
-                    tc_fence_after();
-                    const uint32_t base = saddr(sm.stage[s]);
-                    const uint32_t d = tmem + uint32_t(buf * N);
+                bool ok = true;
+                for (int st = 0; st < nst && ok; ++st) {
+                    const int s = st % kStages;
+                    if (!(ok = mbar_wait(&sm.ready[s], uint32_t((st / kStages) & 1), failed))) break;
 #pragma unroll
-                    for (int q = S::kTerms - 1; q >= 0; --q)
+                    for (int j = 0; j < kSub; ++j) {
+                        const int kb = st * kSub + j, grp = kb >> a.group_shift, buf = grp & 1;
+                        const bool first = (kb & (gb - 1)) == 0;
+                        if (first && grp >= 2 &&
+                            !(ok = mbar_wait(&sm.acce[buf], uint32_t(((grp >> 1) - 1) & 1), failed)))
+                            break;
+                        tc_fence_after();
+                        const uint32_t base = saddr(sm.stage[s]) + j * kATileBytes;
+                        const uint32_t x = saddr(sm.stage[s]) + kSub * kATileBytes + j * S::kXBytes;
+                        const uint32_t d = tmem + uint32_t(buf * N);
 #pragma unroll
-                        for (int k = 0; k < kBK / 16; ++k)
-                            mma_pair(d, smem_desc(base + 32 * k, 16, 1024, 2),
-                                     smem_desc(base + kATileBytes + q * S::kXTermBytes + 32 * k, 16, 1024, 2), idesc,
-                                     first && q == S::kTerms - 1 && k == 0 ? 0u : 1u);
+                        for (int q = S::kTerms - 1; q >= 0; --q)
+#pragma unroll
+                            for (int k = 0; k < kBK / 16; ++k)
+                                mma_pair(d, smem_desc(base + 32 * k, 16, 1024, 2),
+                                         smem_desc(x + q * S::kXTermBytes + 32 * k, 16, 1024, 2), idesc,
+                                         first && q == S::kTerms - 1 && k == 0 ? 0u : 1u);
+                        if ((kb & (gb - 1)) == gb - 1) commit_pair(&sm.accf[buf], mask);
+                    }
                     commit_pair(&sm.empty[s], mask);
-                    if ((kb & (gb - 1)) == gb - 1) commit_pair(&sm.accf[buf], mask);
                 }
                 commit_pair(&sm.done, mask);
                 // no CTA leaves while a draining warp's arrival is on its way to it
@@ -201,9 +215,9 @@ __global__ void __launch_bounds__(kThreads, 1)
             mbar_wait(&sm.done, 0, nullptr);
         } else if (warp == 2 && lane == 0) {
             // tells the even CTA that this CTA's copies of a stage have landed
-            for (int kb = 0; kb < nkb; ++kb) {
-                const int s = kb % kStages;
-                if (!mbar_wait(&sm.xfull[s], uint32_t((kb / kStages) & 1), failed)) break;
+            for (int st = 0; st < nst; ++st) {
+                const int s = st % kStages;
+                if (!mbar_wait(&sm.xfull[s], uint32_t((st / kStages) & 1), failed)) break;
                 fence_proxy_async();
                 mbar_arrive_rank(&sm.ready[s], lead);
             }
@@ -277,25 +291,30 @@ __global__ void __launch_bounds__(kThreads, 1)
         for (int j = 0; j < kMakeAhead; ++j) fetch(j, w[j]);
         bool ok = true;
         int s = 0;
-        uint32_t phase = 1;  // the first round of the ring is free
-        for (int kb0_ = 0; kb0_ < nkb && ok; kb0_ += kMakeAhead) {
+        uint32_t phase = 1;
+        constexpr int kRound = kMakeAhead / kSub;  // stages per turn of the loop
+        for (int st0 = 0; st0 < nst && ok; st0 += kRound) {
 #pragma unroll
-            for (int j = 0; j < kMakeAhead; ++j) {
-                const int kb = kb0_ + j;
-                if (kb >= nkb || !ok) break;
-                if (kb >= kStages && !(ok = mbar_wait(&sm.empty[s], phase, failed))) break;
+            for (int i = 0; i < kRound; ++i) {
+                const int st = st0 + i;
+                if (st >= nst || !ok) break;
+                if (st >= kStages && !(ok = mbar_wait(&sm.empty[s], phase, failed))) break;
                 if (live) {
-                    unsigned char* tile = sm.stage[s];
-                    uint32_t p[4], q[4];
-                    code_pairs<H>(w[j].x, p);
-                    code_pairs<H>(w[j].y, q);
-                    *reinterpret_cast<uint4*>(tile + at0) = make_uint4(p[0], p[2], q[0], q[2]);
-                    *reinterpret_cast<uint4*>(tile + at0 + 8 * 128) = make_uint4(p[1], p[3], q[1], q[3]);
-                    code_pairs<H>(w[j].z, p);
-                    code_pairs<H>(w[j].w, q);
-                    *reinterpret_cast<uint4*>(tile + at1) = make_uint4(p[0], p[2], q[0], q[2]);
-                    *reinterpret_cast<uint4*>(tile + at1 + 8 * 128) = make_uint4(p[1], p[3], q[1], q[3]);
-                    fetch(kb + kMakeAhead, w[j]);
+#pragma unroll
+                    for (int j = 0; j < kSub; ++j) {
+                        unsigned char* tile = sm.stage[s] + j * kATileBytes;
+                        uint4& cw = w[i * kSub + j];
+                        uint32_t p[4], q[4];
+                        code_pairs<H>(cw.x, p);
+                        code_pairs<H>(cw.y, q);
+                        *reinterpret_cast<uint4*>(tile + at0) = make_uint4(p[0], p[2], q[0], q[2]);
+                        *reinterpret_cast<uint4*>(tile + at0 + 8 * 128) = make_uint4(p[1], p[3], q[1], q[3]);
+                        code_pairs<H>(cw.z, p);
+                        code_pairs<H>(cw.w, q);
+                        *reinterpret_cast<uint4*>(tile + at1) = make_uint4(p[0], p[2], q[0], q[2]);
+                        *reinterpret_cast<uint4*>(tile + at1 + 8 * 128) = make_uint4(p[1], p[3], q[1], q[3]);
+                        fetch((st + kRound) * kSub + j, cw);
+                    }
                     fence_proxy_async();
                 }
                 __syncwarp();
