@@ -233,6 +233,7 @@ __global__ void __launch_bounds__(kThreads, 1)
             asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
         }
     }
+    __syncwarp();
     tc_fence_before();
     __syncthreads();
     if (csize > 1) cluster_sync_relaxed();  // the peers' barriers exist before anyone arrives on them
@@ -270,38 +271,32 @@ __global__ void __launch_bounds__(kThreads, 1)
             if (rank == lead) {
                 constexpr uint32_t idesc = instr_desc_f16(kBT, kBN, !kSym);
                 const uint16_t mask = uint16_t(PAIR ? 3u << lead : 0u);
+                const uint32_t left0 = desc_address(saddr(sm.stage[0]), 16);
+                const uint32_t right0 = desc_address(saddr(sm.stage[0]) + 2 * kPlaneBytes, kSym ? 16 : kPlaneBytes);
                 for (int kb = 0; kb < nkb; ++kb) {
                     const int s = kb % kStages, buf = kb & 1;
                     if (kb >= 2 && !mbar_wait(&sm.acce[buf], uint32_t(((kb >> 1) - 1) & 1), failed)) break;
                     if (!mbar_wait(&sm.full[s], uint32_t((kb / kStages) & 1), failed)) break;
                     if (PAIR && !mbar_wait(&sm.ready[s], uint32_t((kb / kStages) & 1), failed)) break;
                     tc_fence_after();
-                    const uint32_t base = saddr(sm.stage[s]);
                     const uint32_t d = tmem + uint32_t(buf * kBN);
-                    uint64_t lh[kBK / 16], ll[kBK / 16], rh[kBK / 16], rl[kBK / 16];
+                    // K-major: 16 binary16 = 32 bytes on along the row; 8-row groups 1024 bytes apart.
+                    // MN-major: 16 K-rows of 128 bytes on; 8-row groups 1024 bytes, 64-column atoms (hi and lo of
+                    // one, then of the next) a plane apart.
+                    constexpr uint32_t kRest = desc_rest(1024, kLayoutSW128);
+                    const uint32_t lh = left0 + uint32_t(s) * (kStageBytes >> 4), ll = lh + (kPlaneBytes >> 4);
+                    const uint32_t rh = right0 + uint32_t(s) * (kStageBytes >> 4),
+                                   rl = rh + ((kSym ? kPlaneBytes : kPlaneBytes / 2) >> 4);
+                    constexpr uint32_t kRight = (kSym ? 32 : 2048) >> 4;
 #pragma unroll
                     for (int k = 0; k < kBK / 16; ++k) {
-                        // K-major: 16 binary16 = 32 bytes on along the row; 8-row groups 1024 bytes apart
-                        lh[k] = smem_desc(base + 32 * k, 16, 1024, kLayoutSW128);
-                        ll[k] = smem_desc(base + kPlaneBytes + 32 * k, 16, 1024, kLayoutSW128);
-                        if constexpr (kSym) {
-                            rh[k] = smem_desc(base + 2 * kPlaneBytes + 32 * k, 16, 1024, kLayoutSW128);
-                            rl[k] = smem_desc(base + 3 * kPlaneBytes + 32 * k, 16, 1024, kLayoutSW128);
-                        } else {
-                            // MN-major: 16 K-rows of 128 bytes on; 8-row groups 1024 bytes, 64-column atoms
-                            // (hi and lo of one, then of the next) a plane apart
-                            rh[k] = smem_desc(base + 2 * kPlaneBytes + 2048 * k, kPlaneBytes, 1024, kLayoutSW128);
-                            rl[k] = smem_desc(base + 2 * kPlaneBytes + kPlaneBytes / 2 + 2048 * k, kPlaneBytes, 1024,
-                                              kLayoutSW128);
-                        }
+                        const uint64_t r = desc_join(rh + k * kRight, kRest);
+                        mma_f16<PAIR>(d, desc_join(ll + 2 * k, kRest), r, idesc, k > 0 ? 1u : 0u);
+                        mma_f16<PAIR>(d, desc_join(lh + 2 * k, kRest), desc_join(rl + k * kRight, kRest), idesc, 1u);
                     }
 #pragma unroll
-                    for (int k = 0; k < kBK / 16; ++k) {
-                        mma_f16<PAIR>(d, ll[k], rh[k], idesc, k > 0 ? 1u : 0u);
-                        mma_f16<PAIR>(d, lh[k], rl[k], idesc, 1u);
-                    }
-#pragma unroll
-                    for (int k = 0; k < kBK / 16; ++k) mma_f16<PAIR>(d, lh[k], rh[k], idesc, 1u);
+                    for (int k = 0; k < kBK / 16; ++k)
+                        mma_f16<PAIR>(d, desc_join(lh + 2 * k, kRest), desc_join(rh + k * kRight, kRest), idesc, 1u);
                     commit<PAIR>(&sm.empty[s], mask);
                     commit<PAIR>(&sm.accf[buf], mask);
                 }
@@ -330,7 +325,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         bool ok = true;
         for (int kb = 0; kb < nkb; ++kb) {
             const int buf = kb & 1;
-            if (!(ok = mbar_wait(&sm.accf[buf], uint32_t((kb >> 1) & 1), failed))) break;
+            if (!(ok = mbar_wait_warp(&sm.accf[buf], uint32_t((kb >> 1) & 1), failed))) break;
             tc_fence_after();
 #pragma unroll
             for (int h = 0; h < kCols / 32; ++h) {
@@ -356,6 +351,7 @@ __global__ void __launch_bounds__(kThreads, 1)
                 *reinterpret_cast<float4*>(row + i) = make_float4(sum[i], sum[i + 1], sum[i + 2], sum[i + 3]);
         }
     }
+    __syncwarp();  // the role warps worked with one lane
     tc_fence_before();
     __syncthreads();
     if (csize > 1) cluster_sync();  // the peers' partial tiles are complete
@@ -468,6 +464,7 @@ __global__ void __launch_bounds__(kThreads, 1)
             }
         }
     }
+    __syncwarp();  // the role warps worked with one lane
     tc_fence_before();
     __syncthreads();
     if (csize > 1) cluster_sync_relaxed();  // no read of a peer's shared memory is outstanding

@@ -33,7 +33,7 @@ constexpr int kDrainWarp0 = 4, kDrainWarps = 8;
 constexpr int kMakeWarp0 = kDrainWarp0 + kDrainWarps, kMakeWarps = 8;  // a row block of the tile each
 constexpr int kThreads = (kMakeWarp0 + kMakeWarps) * 32;
 constexpr int kMakeAhead = 4;  // blocks of codes in flight per warp (whole stages)
-constexpr int kMaxSplits = 4;
+constexpr int kMaxSplits = 2;  // pairs of a cluster; clusters of eight CTAs did not all fit the GPU at once
 // 640 threads launch with 96 registers each; control and making warps give to those that drain
 constexpr uint32_t kRegsControl = 40, kRegsDrain = 168, kRegsMake = 48;
 static_assert(128 * kRegsControl + 256 * kRegsDrain + 256 * kRegsMake <= kThreads * 96, "register split");
@@ -150,6 +150,7 @@ __global__ void __launch_bounds__(kThreads, 1)
                      : "memory");
         asm volatile("tcgen05.relinquish_alloc_permit.cta_group::2.sync.aligned;" ::: "memory");
     }
+    __syncwarp();
     tc_fence_before();
     __syncthreads();
     cluster_sync_relaxed();  // the peers' barriers exist before anyone arrives on them
@@ -180,6 +181,7 @@ __global__ void __launch_bounds__(kThreads, 1)
             if (rank == lead) {
                 constexpr uint32_t idesc = instr_desc_16<H>(256, N);
                 const uint16_t mask = uint16_t(3u << lead);
+                const uint32_t stage0 = desc_address(saddr(sm.stage[0]), 16);
                 bool ok = true;
                 for (int st = 0; st < nst && ok; ++st) {
                     const int s = st % kStages;
@@ -192,16 +194,19 @@ __global__ void __launch_bounds__(kThreads, 1)
                             !(ok = mbar_wait(&sm.acce[buf], uint32_t(((grp >> 1) - 1) & 1), failed)))
                             break;
                         tc_fence_after();
-                        const uint32_t base = saddr(sm.stage[s]) + j * kATileBytes;
-                        const uint32_t x = saddr(sm.stage[s]) + kSub * kATileBytes + j * S::kXBytes;
+                        // K-major: 16 features = 32 bytes on along the row; 8-row groups 1024 bytes apart
+                        constexpr uint32_t kRest = desc_rest(1024, 2);
+                        const uint32_t w = stage0 + uint32_t(s) * (S::kStageBytes >> 4) + j * (kATileBytes >> 4);
+                        const uint32_t x = stage0 + uint32_t(s) * (S::kStageBytes >> 4) +
+                                           ((kSub * kATileBytes + j * S::kXBytes) >> 4);
                         const uint32_t d = tmem + uint32_t(buf * N);
 #pragma unroll
                         for (int q = S::kTerms - 1; q >= 0; --q)
 #pragma unroll
                             for (int k = 0; k < kBK / 16; ++k)
-                                mma_pair(d, smem_desc(base + 32 * k, 16, 1024, 2),
-                                         smem_desc(x + q * S::kXTermBytes + 32 * k, 16, 1024, 2), idesc,
-                                         first && q == S::kTerms - 1 && k == 0 ? 0u : 1u);
+                                mma_pair(d, desc_join(w + 2 * k, kRest),
+                                         desc_join(x + q * (S::kXTermBytes >> 4) + 2 * k, kRest), idesc,
+                                         q == S::kTerms - 1 && k == 0 ? uint32_t(!first) : 1u);
                         if ((kb & (gb - 1)) == gb - 1) commit_pair(&sm.accf[buf], mask);
                     }
                     commit_pair(&sm.empty[s], mask);
@@ -242,7 +247,7 @@ __global__ void __launch_bounds__(kThreads, 1)
             const float s = to_arith<float>(next);
             sc += kQ4Rows;
             if (live && grp + 1 < ngrp) next = *sc;
-            if (!(ok = mbar_wait(&sm.accf[buf], uint32_t((grp >> 1) & 1), failed))) break;
+            if (!(ok = mbar_wait_warp(&sm.accf[buf], uint32_t((grp >> 1) & 1), failed))) break;
             tc_fence_after();
 #pragma unroll
             for (int h = 0; h < kCols / 16; ++h) {
@@ -298,7 +303,7 @@ __global__ void __launch_bounds__(kThreads, 1)
             for (int i = 0; i < kRound; ++i) {
                 const int st = st0 + i;
                 if (st >= nst || !ok) break;
-                if (st >= kStages && !(ok = mbar_wait(&sm.empty[s], phase, failed))) break;
+                if (st >= kStages && !(ok = mbar_wait_warp(&sm.empty[s], phase, failed))) break;
                 if (live) {
 #pragma unroll
                     for (int j = 0; j < kSub; ++j) {
@@ -326,6 +331,7 @@ __global__ void __launch_bounds__(kThreads, 1)
             }
         }
     }
+    __syncwarp();  // the role warps worked with one lane
     tc_fence_before();
     __syncthreads();
     if (a.splits > 1) {
@@ -349,6 +355,7 @@ __global__ void __launch_bounds__(kThreads, 1)
             }
         }
     }
+    __syncwarp();
     cluster_sync_relaxed();  // no arrival, MMA or read targets a CTA that has left
     if (warp == 1) {
         tc_fence_after();

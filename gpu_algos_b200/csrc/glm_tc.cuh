@@ -66,6 +66,13 @@ __device__ __forceinline__ bool mbar_wait(unsigned long long* b, uint32_t parity
     return true;
 }
 
+// The same for a whole warp, which comes out of it converged (what follows -- TMEM loads, an arrival for the
+// warp -- needs that) and of one mind.
+__device__ __forceinline__ bool mbar_wait_warp(unsigned long long* b, uint32_t parity, volatile int* failed) {
+    const bool ok = mbar_wait(b, parity, failed);
+    return __all_sync(0xffffffffu, ok) != 0;
+}
+
 __device__ __forceinline__ void fence_proxy_async() { asm volatile("fence.proxy.async.shared::cta;" ::: "memory"); }
 __device__ __forceinline__ void tc_fence_before() { asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory"); }
 __device__ __forceinline__ void tc_fence_after() { asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory"); }
@@ -78,6 +85,20 @@ __device__ __forceinline__ uint64_t smem_desc(uint32_t addr, uint32_t lbo, uint3
     d |= uint64_t((sbo >> 4) & 0x3FFF) << 32;
     d |= uint64_t(1) << 46;  // descriptor version for sm_100
     d |= uint64_t(layout & 7) << 61;
+    return d;
+}
+
+// The two words of such a descriptor apart: the one with the address, which a loop can add to (in units of 16
+// bytes), and the one that stays.  One thread issues all MMAs, so every instruction it spends on a descriptor
+// is on the path: building whole descriptors per MMA took longer than the MMAs of N < 256.
+// (A shared-memory address carries the CTA's rank in its cluster above the bits a descriptor takes.)
+__device__ __forceinline__ uint32_t desc_address(uint32_t addr, uint32_t lbo) {
+    return ((addr >> 4) & 0x3FFF) | ((lbo >> 4) << 16);
+}
+constexpr uint32_t desc_rest(uint32_t sbo, uint32_t layout) { return (sbo >> 4) | (1u << 14) | (layout << 29); }
+__device__ __forceinline__ uint64_t desc_join(uint32_t address, uint32_t rest) {
+    uint64_t d;
+    asm("mov.b64 %0, {%1, %2};" : "=l"(d) : "r"(address), "r"(rest));
     return d;
 }
 
