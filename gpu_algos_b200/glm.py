@@ -19,7 +19,6 @@ on ``stream``.
 """
 from __future__ import annotations
 
-import contextlib
 import ctypes
 import math
 
@@ -256,21 +255,41 @@ def _matrix_suffix(dtype) -> str:
     return SUFFIX[dtype]
 
 
-@contextlib.contextmanager
-def _launch_on(device, stream):
-    """The tensors' device and the call's stream are current (allocations
-    included) while the library is called; yields the stream's handle."""
-    if stream is not None and stream.device != device:
-        raise ValueError(f"stream is on {stream.device}, the tensors are on {device}")
-    with torch.cuda.device(device):
-        with torch.cuda.stream(stream) if stream is not None else contextlib.nullcontext():
-            yield torch.cuda.current_stream(device).cuda_stream
+def _refuse(t, name: str, shape, dtype, device) -> None:
+    _need(t, name, shape, dtype)
+    raise ValueError(f"{name} is on {t.device}, expected {device}")
 
 
 def _need_on(t: torch.Tensor, name: str, shape, dtype, device) -> None:
-    _need(t, name, shape, dtype)
-    if t.device != device:
-        raise ValueError(f"{name} is on {t.device}, expected {device}")
+    # the checks of _need, in the order that costs a good call least
+    if t.dtype != dtype or t.device != device or t.shape != shape or not t.is_cuda or not t.is_contiguous():
+        _refuse(t, name, shape, dtype, device)
+
+
+def _on(device, stream):
+    """A context in which the tensors' device and the call's stream are
+    current, allocations included; None where they are already."""
+    if stream is None:
+        return None if device.index == torch.cuda.current_device() else torch.cuda.device(device)
+    if stream.device != device:
+        raise ValueError(f"stream is on {stream.device}, the tensors are on {device}")
+    return torch.cuda.stream(stream)
+
+
+def _run(name: str, sfx: str, device, args) -> None:
+    """One call of the library on the current stream of ``device``."""
+    f = _entry.get((name, sfx))
+    if f is None:
+        f = _entry[(name, sfx)] = getattr(capi.lib(), f"{name}_{sfx}")
+    st = f(*args, _raw_stream(device.index))
+    if st != capi.GLMB_OK:
+        capi.check(st, f"{name}_{sfx}")
+
+
+_entry: dict = {}
+# the current stream's handle without building a Stream object around it (2 us of a call)
+_raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream",
+                      lambda index: torch.cuda.current_stream(index).cuda_stream)
 
 
 def _workspace(workspace, device):
@@ -280,7 +299,7 @@ def _workspace(workspace, device):
         raise ValueError(f"workspace is on {workspace.device}, expected {device}")
     if not workspace.is_contiguous():
         raise ValueError("workspace must be contiguous")
-    return workspace.data_ptr(), workspace.numel() * workspace.element_size()
+    return workspace.data_ptr(), workspace.nbytes
 
 
 def _model_dims(M: torch.Tensor, name: str):
@@ -292,7 +311,7 @@ def _model_dims(M: torch.Tensor, name: str):
 def _coefficients(coefficients, steps: int):
     """A host array of 3*steps doubles, or None for the library's own."""
     if coefficients is None:
-        return None
+        return None  # the library checks `steps`
     rows = list(coefficients)
     if len(rows) == 3 and all(isinstance(v, (int, float)) for v in rows):
         rows = [rows] * steps
@@ -314,17 +333,21 @@ def orthogonalize(G, steps: int = 5, coefficients=None, out=None, workspace=None
     ``coefficients``: one (a, b, c) or one per step, by default (3.4445,
     -4.7750, 2.0315), which brings the singular values near 1 in five steps.
     ``out`` may be ``G``."""
-    sfx = _matrix_suffix(G.dtype)
+    sfx, device = _matrix_suffix(G.dtype), G.device
     ntasks, nt, nf = _model_dims(G, "G")
-    _need(G, "G", G.shape, G.dtype)
-    coef = _coefficients(coefficients, int(steps))
-    with _launch_on(G.device, stream) as s:
-        if out is None:
-            out = torch.empty_like(G)
-        _need_on(out, "out", G.shape, G.dtype, G.device)
-        ws_ptr, ws_bytes = _workspace(workspace, G.device)
-        capi.call(f"glmm_orthogonalize_{sfx}", _ptr(G), _ptr(out), nf, nt, ntasks, coef, int(steps), ws_ptr,
-                  ws_bytes, s)
+    _need_on(G, "G", G.shape, G.dtype, device)
+    coef = _coefficients(coefficients, steps)
+    on = _on(device, stream)
+    if on is not None:
+        with on:
+            return orthogonalize(G, steps, coefficients, out, workspace)
+    if out is None:
+        out = torch.empty_like(G)
+    else:
+        _need_on(out, "out", G.shape, G.dtype, device)
+    ws_ptr, ws_bytes = _workspace(workspace, device)
+    _run("glmm_orthogonalize", sfx, device,
+         (G.data_ptr(), out.data_ptr(), nf, nt, ntasks, coef, steps, ws_ptr, ws_bytes))
     return out
 
 
@@ -339,19 +362,23 @@ def orthogonal_step(M, grad, momentum, lr: float, mu: float = 0.95, nesterov: bo
 
     ``grad`` has M's type (as :func:`gradient` returns it); ``scale`` is
     sqrt(max(1, ntargets/nfeatures)) by default.  Returns ``M``."""
-    sfx = _matrix_suffix(M.dtype)
+    sfx, device = _matrix_suffix(M.dtype), M.device
     ntasks, nt, nf = _model_dims(M, "M")
-    _need(M, "M", M.shape, M.dtype)
-    _need_on(grad, "grad", M.shape, M.dtype, M.device)
-    _need_on(momentum, "momentum", M.shape, torch.float32, M.device)
+    _need_on(M, "M", M.shape, M.dtype, device)
+    _need_on(grad, "grad", M.shape, M.dtype, device)
+    _need_on(momentum, "momentum", M.shape, torch.float32, device)
     if scale is None:
         scale = math.sqrt(max(1.0, nt / nf)) if nf > 0 else 1.0
-    coef = _coefficients(coefficients, int(steps))
-    with _launch_on(M.device, stream) as s:
-        ws_ptr, ws_bytes = _workspace(workspace, M.device)
-        capi.call(f"glmm_orthogonal_step_{sfx}", _ptr(M), _ptr(grad), _ptr(momentum), nf, nt, ntasks, float(lr),
-                  float(mu), float(weight_decay), float(scale), capi.STEP_NESTEROV if nesterov else 0, coef,
-                  int(steps), ws_ptr, ws_bytes, s)
+    coef = _coefficients(coefficients, steps)
+    on = _on(device, stream)
+    if on is not None:
+        with on:
+            return orthogonal_step(M, grad, momentum, lr, mu, nesterov, weight_decay, scale, steps, coefficients,
+                                   workspace)
+    ws_ptr, ws_bytes = _workspace(workspace, device)
+    _run("glmm_orthogonal_step", sfx, device,
+         (M.data_ptr(), grad.data_ptr(), momentum.data_ptr(), nf, nt, ntasks, float(lr), float(mu),
+          float(weight_decay), float(scale), capi.STEP_NESTEROV if nesterov else 0, coef, steps, ws_ptr, ws_bytes))
     return M
 
 
@@ -367,8 +394,11 @@ class Q4Model:
         if self.group not in (64, 128):
             raise ValueError(f"group is {group}, expected 64 or 128")
         L = capi.lib()
-        self.codes = torch.empty(L.glmm_q4_codes_bytes(nf, nt, ntasks), dtype=torch.uint8, device=device)
-        self.scales = torch.empty(L.glmm_q4_scales_count(nf, nt, ntasks, self.group), dtype=dtype, device=device)
+        codes = L.glmm_q4_codes_bytes(nf, nt, ntasks)
+        # one allocation; the scales follow the codes, which are a multiple of 512 bytes
+        count = L.glmm_q4_scales_count(nf, nt, ntasks, self.group)
+        held = torch.empty(codes + count * dtype.itemsize, dtype=torch.uint8, device=device)
+        self.codes, self.scales = held[:codes], held[codes:].view(dtype)
 
     @property
     def device(self):
@@ -379,27 +409,38 @@ def quantize_q4(M, group: int = 128, out=None, stream=None) -> Q4Model:
     """``M`` in 4 bits: per target and group of 64 or 128 features a scale
     s = max|w|/7 (rounded to M's type) and codes q = w/s rounded to the nearest
     of -7..7, ties to even.  ``out``: a Q4Model of the same shape to overwrite."""
-    sfx = _matrix_suffix(M.dtype)
+    sfx, device = _matrix_suffix(M.dtype), M.device
     ntasks, nt, nf = _model_dims(M, "M")
-    _need(M, "M", M.shape, M.dtype)
-    with _launch_on(M.device, stream) as s:
-        if out is None:
-            out = Q4Model(M.shape, M.dtype, group, M.device)
-        if (out.shape, out.dtype, out.group, out.device) != (tuple(M.shape), M.dtype, group, M.device):
-            raise ValueError("out was made for another shape, dtype, group or device")
-        capi.call(f"glmm_quantize_q4_{sfx}", _ptr(M), _ptr(out.codes), _ptr(out.scales), nf, nt, ntasks, out.group, s)
+    _need_on(M, "M", M.shape, M.dtype, device)
+    on = _on(device, stream)
+    if on is not None:
+        with on:
+            return quantize_q4(M, group, out)
+    if out is None:
+        out = Q4Model(M.shape, M.dtype, group, device)
+    elif (out.shape, out.dtype, out.group, out.device) != (tuple(M.shape), M.dtype, group, device):
+        raise ValueError("out was made for another shape, dtype, group or device")
+    _run("glmm_quantize_q4", sfx, device,
+         (M.data_ptr(), out.codes.data_ptr(), out.scales.data_ptr(), nf, nt, ntasks, out.group))
     return out
 
 
 def dequantize_q4(model: Q4Model, out=None, stream=None):
     """The weights q*s of a :class:`Q4Model`, rounded to its dtype."""
     ntasks, nt, nf = model.shape
-    with _launch_on(model.device, stream) as s:
-        if out is None:
-            out = torch.empty(model.shape, dtype=model.dtype, device=model.device)
-        _need_on(out, "out", model.shape, model.dtype, model.device)
-        capi.call(f"glmm_dequantize_q4_{SUFFIX[model.dtype]}", _ptr(model.codes), _ptr(model.scales), _ptr(out), nf,
-                  nt, ntasks, model.group, s)
+    device = model.device
+    if device.type != "cuda":
+        raise ValueError("model must be on a CUDA device")
+    on = _on(device, stream)
+    if on is not None:
+        with on:
+            return dequantize_q4(model, out)
+    if out is None:
+        out = torch.empty(model.shape, dtype=model.dtype, device=device)
+    else:
+        _need_on(out, "out", model.shape, model.dtype, device)
+    _run("glmm_dequantize_q4", SUFFIX[model.dtype], device,
+         (model.codes.data_ptr(), model.scales.data_ptr(), out.data_ptr(), nf, nt, ntasks, model.group))
     return out
 
 
@@ -413,17 +454,22 @@ def predict_q4(X, model: Q4Model, out=None, workspace=None, stream=None):
     """:func:`predict` from a :class:`Q4Model`: Yhat[obs, task, t] = sum_f
     q[task, t, f]*s X[obs, task, f], from one observation to many; the products
     are those of the exact weights q*s, sums are float32."""
-    sfx = _matrix_suffix(model.dtype)
     ntasks, nt, nf = model.shape
+    dtype, device = model.dtype, model.device
     if X.dim() != 3:
         raise ValueError(f"X has shape {tuple(X.shape)}, expected (nobs, ntasks, nfeatures)")
     nobs = X.shape[0]
-    _need_on(X, "X", (nobs, ntasks, nf), model.dtype, model.device)
-    with _launch_on(model.device, stream) as s:
-        if out is None:
-            out = torch.empty((nobs, ntasks, nt), dtype=X.dtype, device=X.device)
-        _need_on(out, "out", (nobs, ntasks, nt), X.dtype, X.device)
-        ws_ptr, ws_bytes = _workspace(workspace, X.device)
-        capi.call(f"glmm_predict_q4_{sfx}", _ptr(X), _ptr(model.codes), _ptr(model.scales), _ptr(out), nf, nt,
-                  ntasks, nobs, model.group, ws_ptr, ws_bytes, s)
+    _need_on(X, "X", (nobs, ntasks, nf), dtype, device)
+    on = _on(device, stream)
+    if on is not None:
+        with on:
+            return predict_q4(X, model, out, workspace)
+    if out is None:
+        out = torch.empty((nobs, ntasks, nt), dtype=dtype, device=device)
+    else:
+        _need_on(out, "out", (nobs, ntasks, nt), dtype, device)
+    ws_ptr, ws_bytes = _workspace(workspace, device)
+    _run("glmm_predict_q4", SUFFIX[dtype], device,
+         (X.data_ptr(), model.codes.data_ptr(), model.scales.data_ptr(), out.data_ptr(), nf, nt, ntasks, nobs,
+          model.group, ws_ptr, ws_bytes))
     return out
