@@ -21,12 +21,12 @@ inline unsigned warp_grid(int64_t warps) {
     return unsigned(std::max<int64_t>(1, std::min<int64_t>(int64_t(sm_count()) * 32, (warps + kWarps - 1) / kWarps)));
 }
 
-// ---- rows of sixteen features -------------------------------------------------
+// ---- a lane's sixteen features of a row ---------------------------------------
 //
-// Lane 4g + c of a warp works on features 16c..16c+15 of a 64-feature block of
-// rows g and g + 8.  Where rows start on 16 bytes (`vec`) it moves its sixteen
-// as 16-byte pieces; elsewhere the warp moves each row's 64 features side by
-// side and passes them through shared memory.
+// Lane 4g + c of a warp works on features 16k + 4c .. + 3, k = 0..3, of a
+// 64-feature block of rows g and g + 8.  Where rows start on, and are made of,
+// whole pieces of four (`vec`) it moves them as such; elsewhere the warp moves
+// each row's 64 features side by side and passes them through shared memory.
 
 constexpr int kTileLd = kQ4Cols + 8;  // elements of T between the rows of a staged block
 
@@ -35,22 +35,21 @@ struct RowTile {
     alignas(16) T at[kQ4Rows][kTileLd];
 };
 
-// v = features f0 + 16c.. of rows row0 + g and row0 + g + 8 (zero past nf and past `rows`) of M[.][nf].
+// v[h][4k + j] = feature f0 + 16k + 4c + j of row row0 + g + 8h (zero past nf and past `rows`) of M[.][nf].
 template <typename T>
 __device__ __forceinline__ void load_rows(const T* M, int64_t row0, int rows, int64_t f0, int64_t nf, bool vec,
                                           RowTile<T>& tile, float (&v)[2][16]) {
-    constexpr int kPer = 16 / sizeof(T);
     const int lane = threadIdx.x & 31, g = lane >> 2, c = lane & 3;
     if (vec) {
 #pragma unroll
         for (int h = 0; h < 2; ++h)
 #pragma unroll
-            for (int i = 0; i < 16; i += kPer) {
-                T t[kPer] = {};
-                if (g + 8 * h < rows && f0 + 16 * c + i < nf)
-                    VecLoad<T, kPer>::load(M + (row0 + g + 8 * h) * nf + f0 + 16 * c + i, t);
+            for (int k = 0; k < 4; ++k) {
+                T t[4] = {};
+                if (g + 8 * h < rows && f0 + 16 * k + 4 * c < nf)
+                    VecLoad<T, 4>::load(M + (row0 + g + 8 * h) * nf + f0 + 16 * k + 4 * c, t);
 #pragma unroll
-                for (int j = 0; j < kPer; ++j) v[h][i + j] = to_arith<float>(t[j]);
+                for (int j = 0; j < 4; ++j) v[h][4 * k + j] = to_arith<float>(t[j]);
             }
     } else {
         __syncwarp();
@@ -65,12 +64,8 @@ __device__ __forceinline__ void load_rows(const T* M, int64_t row0, int rows, in
 #pragma unroll
         for (int h = 0; h < 2; ++h)
 #pragma unroll
-            for (int i = 0; i < 16; i += kPer) {
-                alignas(16) T t[kPer];
-                *reinterpret_cast<uint4*>(t) = *reinterpret_cast<const uint4*>(&tile.at[g + 8 * h][16 * c + i]);
-#pragma unroll
-                for (int j = 0; j < kPer; ++j) v[h][i + j] = to_arith<float>(t[j]);
-            }
+            for (int i = 0; i < 16; ++i)
+                v[h][i] = to_arith<float>(tile.at[g + 8 * h][16 * (i >> 2) + 4 * c + (i & 3)]);
     }
 }
 
@@ -80,17 +75,26 @@ __device__ __forceinline__ float max_abs_nan(float a, float b) {
     return r;
 }
 
-// q + 8 with q = w / s rounded to the nearest whole number, ties to even, for |w / s| < 7.5 and s > 0.  The
-// float product w * (1/s) can be off by an ulp and land on the wrong side of a border, so the remainder
-// d = w - q*s decides: it is exact in float (w and q*s are multiples of ulp(s)/2 when q != 0, and |d| is s/2
-// or so).  `half` is s/2 and `below` the next float towards zero, the limits for even and for odd q.
+// w / s rounded to the nearest whole number q, ties to even, for |w / s| < 7.5 and s > 0: returned as the bits
+// of the float kOne + q, whose low bits are q's.
+constexpr float kOne = 12582912.0f;  // 1.5 * 2^23: adding it rounds to a whole number
+template <typename T>
 __device__ __forceinline__ uint32_t nearest_code(float w, float s, float inv, float half, float below) {
-    constexpr float kOne = 12582912.0f;  // 1.5 * 2^23: adding it rounds to a whole number, found in the low bits
-    const float m = fmaf(w, inv, kOne);
-    const float d = fmaf(kOne - m, s, w);
-    const int bits = __float_as_int(m);
-    const int step = (__float_as_int(d) >> 31) | 1;
-    return uint32_t(bits + 8 + (fabsf(d) > ((bits & 1) != 0 ? below : half) ? step : 0)) & 15u;
+    if constexpr (std::is_same_v<T, float>) {
+        // The float quotient can be off by an ulp and land on the wrong side of a border, so the remainder
+        // d = w - q*s decides: it is exact in float (w and q*s are multiples of ulp(s)/2 when q != 0, and |d|
+        // is s/2 or so).  `half` is s/2 and `below` the next float towards zero, the limits for even and odd q.
+        const float m = fmaf(w, inv, kOne);
+        const float d = fmaf(kOne - m, s, w);
+        const int bits = __float_as_int(m);
+        const int step = (__float_as_int(d) >> 31) | 1;
+        return uint32_t(bits + (fabsf(d) > ((bits & 1) != 0 ? below : half) ? step : 0));
+    } else {
+        // One correction makes the quotient the float nearest to w / s, which is w / s itself on a border; of
+        // 16-bit w and s (11 bits at most) any other quotient is 2^-12 of it or more away from one.
+        const float t = w * inv;
+        return __float_as_uint(fmaf(fmaf(-t, s, w), inv, t) + kOne);
+    }
 }
 
 // One warp per (task, 16 targets, group).  A group's largest magnitude is a maximum over the four lanes of
@@ -152,12 +156,14 @@ __global__ void __launch_bounds__(kThreads)
             uint32_t word[4];
 #pragma unroll
             for (int k = 0; k < 4; ++k) {
-                word[k] = 0;
+                // the sum of (q + 8) 2^shift, modulo 2^32, from the bits of kOne + q
+                word[k] = 0x11111111u * (8u - __float_as_uint(kOne));
 #pragma unroll
                 for (int p = 0; p < 8; ++p) {
                     // p: pair 0..3 = (g, f), (g+8, f), (g, f+2), (g+8, f+2); 4..7 the same of f + 1
                     const int h = p & 1, i = 4 * k + (p & 2) + (p >> 2);
-                    word[k] |= nearest_code(v[b][h][i], s[h], inv[h], half[h], below[h]) << (4 * (p & 3) + 16 * (p >> 2));
+                    word[k] += nearest_code<T>(v[b][h][i], s[h], inv[h], half[h], below[h])
+                               << (4 * (p & 3) + 16 * (p >> 2));
                 }
             }
             codes[((task * nrb + rb) * ncb + cb) * 32 + lane] = make_uint4(word[0], word[1], word[2], word[3]);
@@ -178,6 +184,13 @@ __device__ __forceinline__ void scaled_pair(uint32_t pair, T s, uint32_t* dst) {
         const __nv_bfloat162 v = __hmul2(*reinterpret_cast<const __nv_bfloat162*>(&pair), __bfloat162bfloat162(s));
         dst[0] = *reinterpret_cast<const uint32_t*>(&v);
     }
+}
+
+// Four elements of T from the words that hold them.
+template <typename T>
+__device__ __forceinline__ void store_piece(T* dst, const uint32_t* w) {
+    if constexpr (sizeof(T) == 4) *reinterpret_cast<uint4*>(dst) = make_uint4(w[0], w[1], w[2], w[3]);
+    else *reinterpret_cast<uint2*>(dst) = make_uint2(w[0], w[1]);
 }
 
 // One warp per block of codes: M = q*s, rounded to T.
@@ -209,12 +222,10 @@ __global__ void __launch_bounds__(kThreads)
 #pragma unroll
             for (int h = 0; h < 2; ++h) {
                 if (g + 8 * h >= rows) continue;
-                T* dst = M + (row0 + g + 8 * h) * nf + f0 + 16 * c;
+                T* dst = M + (row0 + g + 8 * h) * nf + f0 + 4 * c;
 #pragma unroll
-                for (int i = 0; i < kWords; i += 4)
-                    if (f0 + 16 * c + i * int(4 / sizeof(T)) < nf)
-                        *reinterpret_cast<uint4*>(reinterpret_cast<uint32_t*>(dst) + i) =
-                            make_uint4(out[h][i], out[h][i + 1], out[h][i + 2], out[h][i + 3]);
+                for (int k = 0; k < 4; ++k)
+                    if (f0 + 16 * k + 4 * c < nf) store_piece(dst + 16 * k, &out[h][k * kWords / 4]);
             }
         } else {
             RowTile<T>& tile = tiles[warp];
@@ -222,9 +233,7 @@ __global__ void __launch_bounds__(kThreads)
 #pragma unroll
             for (int h = 0; h < 2; ++h)
 #pragma unroll
-                for (int i = 0; i < kWords; i += 4)
-                    *reinterpret_cast<uint4*>(reinterpret_cast<uint32_t*>(&tile.at[g + 8 * h][16 * c]) + i) =
-                        make_uint4(out[h][i], out[h][i + 1], out[h][i + 2], out[h][i + 3]);
+                for (int k = 0; k < 4; ++k) store_piece(&tile.at[g + 8 * h][16 * k + 4 * c], &out[h][k * kWords / 4]);
             __syncwarp();
 #pragma unroll 4
             for (int r = 0; r < kQ4Rows; ++r)
@@ -239,12 +248,12 @@ __global__ void __launch_bounds__(kThreads)
 
 // ---- a few observations: the stream of the codes ------------------------------
 //
-// Bound by HBM: half a byte a weight, so with 1 to 8 observations the codes
+// Bound by HBM: half a byte a weight, so with 1 to 16 observations the codes
 // are nearly all that moves.  A warp takes a block of 16 targets x 64 features
 // per step: one 16-byte load per lane is the block's four tensor-core
 // fragments (mma.m16n8k16, weights as the 16-row operand), made into whole
 // numbers of X's 16-bit type in registers, so a fragment costs the same for
-// one observation as for eight; products of 16-bit values are exact and sums
+// one observation as for eight (two fragments' columns for nine to sixteen); products of 16-bit values are exact and sums
 // float.  A block's sums are scaled and added to the warp's totals.  float
 // observations are three bfloat16 terms (8 bits each, together all 24), each
 // with its own products.
@@ -258,11 +267,10 @@ __global__ void __launch_bounds__(kThreads)
 // features out over the CTAs of a cluster as well.
 
 constexpr int kStreamWarps = 16, kStreamThreads = kStreamWarps * 32;
-constexpr int kStreamObs = 8;     // columns of a fragment
 constexpr int kStreamAhead = 4;   // pairs of blocks (128 features) in flight per warp
 constexpr int kStreamRows = 16;   // row blocks a CTA works on together
 constexpr int kSlots = kStreamRows / kStreamWarps + 3;  // row blocks one warp's run can touch
-constexpr int kSlotLd = kQ4Rows + 1, kSlotFloats = kStreamObs * kSlotLd;
+constexpr int kSlotLd = kQ4Rows + 1;
 
 template <typename H>
 __device__ __forceinline__ void mma_16816(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
@@ -291,36 +299,37 @@ struct StreamArgs {
 };
 
 // Where things lie in shared memory: features [term][obs], scales [row block][group], sums [warp][slot].
-template <typename T>
+template <typename T, int NT>
 struct StreamLayout {
     static constexpr int kTerms = Split16<T>::kTerms;
+    static constexpr int kSlotFloats = 8 * NT * kSlotLd;
     int row_bytes, scales_ld;   // of one observation's features; scales of one row block (at most)
     int scales_at, slots_at, bytes;
-    // 16 past a multiple of 128: the rows that eight lanes read together meet no bank twice
+    // 32 past a multiple of 128: the rows that sixteen lanes read together meet no bank twice
     __host__ __device__ StreamLayout(int chunk, int obs, int rows, int group_shift)
-        : row_bytes(chunk * (kQ4Cols * 2) + 16), scales_ld((chunk >> group_shift) * kQ4Rows) {
+        : row_bytes(chunk * (kQ4Cols * 2) + 32), scales_ld((chunk >> group_shift) * kQ4Rows) {
         scales_at = kTerms * obs * row_bytes;
         slots_at = (scales_at + rows * scales_ld * int(sizeof(T)) + 15) / 16 * 16;
         bytes = slots_at + kStreamWarps * kSlots * kSlotFloats * 4;
     }
 };
 
-// GROUPS: groups in 128 features.  FLAT: the CTA takes all of its row blocks' features at once, so that the
+// NT: fragments of eight observations.  GROUPS: groups in 128 features.  FLAT: the CTA takes all of its row blocks' features at once, so that the
 // codes of its row blocks lie end to end.
-template <typename T, int GROUPS, bool FLAT>
+template <typename T, int NT, int GROUPS, bool FLAT>
 __global__ void __launch_bounds__(kStreamThreads, 1)
     q4_stream_kernel(const T* __restrict__ X, const uint4* __restrict__ codes, const T* __restrict__ scales,
                      T* __restrict__ Yhat, StreamArgs a) {
     using H = typename Split16<T>::Type;
-    constexpr int kTerms = Split16<T>::kTerms;
+    constexpr int kTerms = Split16<T>::kTerms, kObs = 8 * NT, kSlotFloats = StreamLayout<T, NT>::kSlotFloats;
     extern __shared__ __align__(16) unsigned char smem_raw[];
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, c = lane & 3;
     const int rank = int(blockIdx.x) & ((1 << a.ranks_log2) - 1), ranks = 1 << a.ranks_log2;
-    const int64_t task = a.task0 + blockIdx.y, obs0 = int64_t(blockIdx.z) * kStreamObs;
-    const int obs_here = int(min(int64_t(kStreamObs), a.nobs - obs0));
+    const int64_t task = a.task0 + blockIdx.y, obs0 = int64_t(blockIdx.z) * kObs;
+    const int obs_here = int(min(int64_t(kObs), a.nobs - obs0));
     const int rb_begin = (int(blockIdx.x) >> a.ranks_log2) * a.rows, rb_end = min(a.nrb, rb_begin + a.rows);
     const int cb_begin = rank * a.per_rank, cb_end = min(a.ncb, cb_begin + a.per_rank);
-    const StreamLayout<T> at(a.chunk, obs_here, min(a.rows, kStreamRows), a.group_shift);
+    const StreamLayout<T, NT> at(a.chunk, obs_here, min(a.rows, kStreamRows), a.group_shift);
     T* const sm_scales = reinterpret_cast<T*>(smem_raw + at.scales_at);
     float* const slots = reinterpret_cast<float*>(smem_raw + at.slots_at);
 
@@ -402,25 +411,33 @@ __global__ void __launch_bounds__(kStreamThreads, 1)
             __syncthreads();
 
             // observations past the last one read another's row; their columns are not stored
-            const unsigned char* const x0 = smem_raw + min(g, obs_here - 1) * at.row_bytes + 32 * c;
-            const unsigned char* x = x0 + col0 * (kQ4Cols * 4);
+            const unsigned char* x[NT];
+#pragma unroll
+            for (int n = 0; n < NT; ++n) x[n] = smem_raw + min(8 * n + g, obs_here - 1) * at.row_bytes + 8 * c;
+            int col = col0 * (kQ4Cols * 4);  // bytes
             const T* sc = sm_scales + run0 * (GROUPS * kQ4Rows) + 2 * g;
             const int term_bytes = obs_here * at.row_bytes;
-            float total[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+            float total[NT][4] = {};
             auto flush = [&] {
-                float* slot = my_slots + (row - first_row) * kSlotFloats + 2 * c * kSlotLd + g;
-                slot[0] += total[0];
-                slot[kSlotLd] += total[1];
-                slot[8] += total[2];
-                slot[kSlotLd + 8] += total[3];
+#pragma unroll
+                for (int n = 0; n < NT; ++n) {
+                    float* slot = my_slots + (row - first_row) * kSlotFloats + (8 * n + 2 * c) * kSlotLd + g;
+                    slot[0] += total[n][0];
+                    slot[kSlotLd] += total[n][1];
+                    slot[8] += total[n][2];
+                    slot[kSlotLd + 8] += total[n][3];
+                }
             };
-            auto add = [&](const float (&acc)[4], const T* at_scale) {
+            auto add = [&](const float (&acc)[NT][4], const T* at_scale) {
                 const Pair<T> s = *reinterpret_cast<const Pair<T>*>(at_scale);
                 const float s0 = to_arith<float>(s.first), s1 = to_arith<float>(s.second);
-                total[0] = fmaf(s0, acc[0], total[0]);
-                total[1] = fmaf(s0, acc[1], total[1]);
-                total[2] = fmaf(s1, acc[2], total[2]);
-                total[3] = fmaf(s1, acc[3], total[3]);
+#pragma unroll
+                for (int n = 0; n < NT; ++n) {
+                    total[n][0] = fmaf(s0, acc[n][0], total[n][0]);
+                    total[n][1] = fmaf(s0, acc[n][1], total[n][1]);
+                    total[n][2] = fmaf(s1, acc[n][2], total[n][2]);
+                    total[n][3] = fmaf(s1, acc[n][3], total[n][3]);
+                }
             };
             for (int left = run1 - run0; left > 0; left -= kStreamAhead) {
 #pragma unroll
@@ -435,31 +452,34 @@ __global__ void __launch_bounds__(kStreamThreads, 1)
                         code_pairs<H>(w[j][h].w, frag[h][3]);
                     }
                     fetch(w[j]);
-                    float acc[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+                    float acc[NT][4] = {};
 #pragma unroll
                     for (int h = 0; h < 2; ++h) {
 #pragma unroll
-                        for (int q = kTerms - 1; q >= 0; --q) {
-                            const uint4* xv = reinterpret_cast<const uint4*>(x + q * term_bytes + h * (kQ4Cols * 2));
-                            const uint4 lo = xv[0], hi = xv[1];
-                            mma_16816<H>(acc, frag[h][0], lo.x, lo.y);
-                            mma_16816<H>(acc, frag[h][1], lo.z, lo.w);
-                            mma_16816<H>(acc, frag[h][2], hi.x, hi.y);
-                            mma_16816<H>(acc, frag[h][3], hi.z, hi.w);
-                        }
+                        for (int n = 0; n < NT; ++n)
+#pragma unroll
+                            for (int q = kTerms - 1; q >= 0; --q)
+#pragma unroll
+                                for (int k = 0; k < 4; ++k) {
+                                    const uint2 xv = *reinterpret_cast<const uint2*>(
+                                        x[n] + col + q * term_bytes + h * (kQ4Cols * 2) + 32 * k);
+                                    mma_16816<H>(acc[n], frag[h][k], xv.x, xv.y);
+                                }
                         if (GROUPS == 2) {
                             add(acc, sc + h * kQ4Rows);
-                            acc[0] = acc[1] = acc[2] = acc[3] = 0.0f;
+#pragma unroll
+                            for (int n = 0; n < NT; ++n) acc[n][0] = acc[n][1] = acc[n][2] = acc[n][3] = 0.0f;
                         }
                     }
                     if (GROUPS == 1) add(acc, sc);
-                    x += kQ4Cols * 4;
+                    col += kQ4Cols * 4;
                     sc += GROUPS * kQ4Rows;
                     if (--left_in_row == 0) {
                         flush();
-                        total[0] = total[1] = total[2] = total[3] = 0.0f;
+#pragma unroll
+                        for (int n = 0; n < NT; ++n) total[n][0] = total[n][1] = total[n][2] = total[n][3] = 0.0f;
                         left_in_row = pairs;
-                        x = x0;
+                        col = 0;
                         ++row;
                     }
                 }
@@ -489,11 +509,11 @@ __global__ void __launch_bounds__(kStreamThreads, 1)
     }
 }
 
-template <typename T>
+template <typename T, int NT>
 int stream_predict(const T* X, const void* codes, const T* scales, T* Yhat, StreamArgs a, cudaStream_t stream) {
     constexpr size_t kRoom = size_t(224) * 1024;
-    const int obs = int(std::min<int64_t>(kStreamObs, a.nobs));
-    const int64_t obs_tiles = (a.nobs + kStreamObs - 1) / kStreamObs, sms = sm_count();
+    const int obs = int(std::min<int64_t>(8 * NT, a.nobs));
+    const int64_t obs_tiles = (a.nobs + 8 * NT - 1) / (8 * NT), sms = sm_count();
     // CTAs for a task's row blocks, one to an SM
     const int64_t ctas = std::max<int64_t>(1, sms / std::min(sms, a.ntasks * obs_tiles));
     a.rows = int((a.nrb + ctas - 1) / ctas);
@@ -506,12 +526,12 @@ int stream_predict(const T* X, const void* codes, const T* scales, T* Yhat, Stre
     a.per_rank = ((a.ncb + ranks - 1) / ranks + 1) / 2 * 2;
     // the longest run of features that leaves room for the scales and sums
     a.chunk = a.per_rank;
-    while (size_t(StreamLayout<T>(a.chunk, obs, rows, a.group_shift).bytes) > kRoom) a.chunk = (a.chunk / 2 + 1) / 2 * 2;
+    while (size_t(StreamLayout<T, NT>(a.chunk, obs, rows, a.group_shift).bytes) > kRoom) a.chunk = (a.chunk / 2 + 1) / 2 * 2;
     const bool flat = a.chunk >= a.ncb;
     static std::atomic<uint64_t> attr[4];
     void (*const kernels[4])(const T*, const uint4*, const T*, T*, StreamArgs) = {
-        q4_stream_kernel<T, 1, false>, q4_stream_kernel<T, 1, true>, q4_stream_kernel<T, 2, false>,
-        q4_stream_kernel<T, 2, true>};
+        q4_stream_kernel<T, NT, 1, false>, q4_stream_kernel<T, NT, 1, true>, q4_stream_kernel<T, NT, 2, false>,
+        q4_stream_kernel<T, NT, 2, true>};
     const int which = (a.group_shift == 0 ? 2 : 0) + (flat ? 1 : 0);
     const auto kernel = kernels[which];
     cudaError_t e = set_smem_limit_once(attr[which], kernel, kRoom);
@@ -519,7 +539,7 @@ int stream_predict(const T* X, const void* codes, const T* scales, T* Yhat, Stre
     if (obs_tiles > 65535 || (groups << a.ranks_log2) > 0x7fffffff) return GLMB_ERR_TOO_LARGE;
     cudaLaunchConfig_t cfg = {};
     cfg.blockDim = dim3(kStreamThreads);
-    cfg.dynamicSmemBytes = size_t(StreamLayout<T>(a.chunk, obs, rows, a.group_shift).bytes);
+    cfg.dynamicSmemBytes = size_t(StreamLayout<T, NT>(a.chunk, obs, rows, a.group_shift).bytes);
     cfg.stream = stream;
     cudaLaunchAttribute at[1];
     at[0].id = cudaLaunchAttributeClusterDimension;
@@ -537,9 +557,10 @@ int stream_predict(const T* X, const void* codes, const T* scales, T* Yhat, Stre
     return launch_status();
 }
 
+// Whether rows of nf elements from p on start on, and are made of, whole pieces of `bytes`.
 template <typename T>
-bool whole_vectors(const T* p, int64_t nf) {
-    return (reinterpret_cast<uintptr_t>(p) & 15u) == 0 && nf % int64_t(16 / sizeof(T)) == 0;
+bool whole_pieces(const T* p, int64_t nf, size_t bytes) {
+    return (reinterpret_cast<uintptr_t>(p) & (bytes - 1)) == 0 && nf % int64_t(bytes / sizeof(T)) == 0;
 }
 
 }  // namespace
@@ -551,7 +572,7 @@ int q4_quantize(const T* M, void* codes, T* scales, int64_t nf, int64_t nt, int6
     const int64_t total = ntasks * nrb * ng;
     auto kernel = group == 64 ? q4_quantize_kernel<T, 64> : q4_quantize_kernel<T, 128>;
     kernel<<<warp_grid(total), kThreads, 0, stream>>>(M, static_cast<uint4*>(codes), scales, nf, nt, nrb, ncb, ng,
-                                                      total, whole_vectors(M, nf));
+                                                      total, whole_pieces(M, nf, 4 * sizeof(T)));
     count_launch();
     return launch_status();
 }
@@ -562,13 +583,13 @@ int q4_dequantize(const void* codes, const T* scales, T* M, int64_t nf, int64_t 
     const int64_t nrb = q4_row_blocks(nt), ncb = q4_col_blocks(nf), ng = q4_groups(nf, group);
     const int64_t total = ntasks * nrb * ncb;
     q4_dequantize_kernel<T><<<warp_grid(total), kThreads, 0, stream>>>(
-        static_cast<const uint4*>(codes), scales, M, nf, nt, nrb, ncb, ng, group == 64 ? 6 : 7, total, whole_vectors(M, nf));
+        static_cast<const uint4*>(codes), scales, M, nf, nt, nrb, ncb, ng, group == 64 ? 6 : 7, total, whole_pieces(M, nf, 4 * sizeof(T)));
     count_launch();
     return launch_status();
 }
 
-// Up to this many observations go through the stream kernel (one pass over the codes per eight of them).
-constexpr int64_t kStreamMost = 8;
+// Up to this many observations go through the stream kernel.
+constexpr int64_t kStreamMost = 16;
 
 template <typename T>
 size_t q4_predict_workspace(int64_t nf, int64_t nt, int64_t ntasks, int64_t nobs, int group) {
@@ -582,13 +603,14 @@ int q4_predict(const T* X, const void* codes, const T* scales, T* Yhat, int64_t 
     if (nrb > (1 << 27) || ncb > (1 << 20)) return GLMB_ERR_TOO_LARGE;
     if (nobs > kStreamMost) {
         set_last_path("q4_tile");
-        return q4_tile_predict<T>(X, codes, scales, Yhat, nf, nt, ntasks, nobs, group, whole_vectors(X, nf), ws,
+        return q4_tile_predict<T>(X, codes, scales, Yhat, nf, nt, ntasks, nobs, group, whole_pieces(X, nf, 16), ws,
                                   ws_bytes, stream);
     }
     StreamArgs a{nf, nt, ntasks, nobs, 0, int(nrb), int(ncb), int(ng), 0, 0, 0, group == 64 ? 0 : 1, 0,
-                 whole_vectors(X, nf)};
+                 whole_pieces(X, nf, 16)};
     set_last_path("q4_stream");
-    return stream_predict<T>(X, codes, scales, Yhat, a, stream);
+    if (nobs <= 8) return stream_predict<T, 1>(X, codes, scales, Yhat, a, stream);
+    return stream_predict<T, 2>(X, codes, scales, Yhat, a, stream);
 }
 
 #define GLMB_INSTANTIATE_Q4(T)                                                                                \

@@ -283,8 +283,14 @@ __global__ void __launch_bounds__(kThreads, 1)
         const int64_t rb = m0 / kQ4Rows + r;
         const bool live = rb < a.nrb;  // rows past the last target are not stored and may hold anything
         const uint4* src = codes + ((task * a.nrb + (live ? rb : 0)) * a.ncb + kb0) * 32 + lane;
-        const uint32_t row = uint32_t((16 * r + g) * 128), at0 = row + uint32_t(((2 * c) ^ g) * 16),
-                       at1 = row + uint32_t(((2 * c + 1) ^ g) * 16);
+        // Word k is four features -- eight bytes -- of row g (and of row g + 8) at feature 16 k + 4 c: half of the
+        // 16-byte chunk 2 k + c / 2, which the swizzle puts at that number xor g.  Lanes of odd g take the words
+        // two on, so that the sixteen lanes of a store meet no bank twice.
+        const uint32_t row = uint32_t((16 * r + g) * 128 + 8 * (c & 1));
+        const bool odd = (g & 1) != 0;
+        uint32_t at[4];
+#pragma unroll
+        for (int k = 0; k < 4; ++k) at[k] = row + uint32_t(((2 * (k ^ (odd ? 2 : 0)) + (c >> 1)) ^ g) * 16);
         uint4 w[kMakeAhead];
         auto fetch = [&](int kb, uint4& cw) {
             if (live && kb < nkb)
@@ -309,15 +315,15 @@ __global__ void __launch_bounds__(kThreads, 1)
                     for (int j = 0; j < kSub; ++j) {
                         unsigned char* tile = sm.stage[s] + j * kATileBytes;
                         uint4& cw = w[i * kSub + j];
-                        uint32_t p[4], q[4];
-                        code_pairs<H>(cw.x, p);
-                        code_pairs<H>(cw.y, q);
-                        *reinterpret_cast<uint4*>(tile + at0) = make_uint4(p[0], p[2], q[0], q[2]);
-                        *reinterpret_cast<uint4*>(tile + at0 + 8 * 128) = make_uint4(p[1], p[3], q[1], q[3]);
-                        code_pairs<H>(cw.z, p);
-                        code_pairs<H>(cw.w, q);
-                        *reinterpret_cast<uint4*>(tile + at1) = make_uint4(p[0], p[2], q[0], q[2]);
-                        *reinterpret_cast<uint4*>(tile + at1 + 8 * 128) = make_uint4(p[1], p[3], q[1], q[3]);
+                        const uint32_t word[4] = {odd ? cw.z : cw.x, odd ? cw.w : cw.y, odd ? cw.x : cw.z,
+                                                  odd ? cw.y : cw.w};
+#pragma unroll
+                        for (int k = 0; k < 4; ++k) {
+                            uint32_t p[4];
+                            code_pairs<H>(word[k], p);
+                            *reinterpret_cast<uint2*>(tile + at[k]) = make_uint2(p[0], p[2]);
+                            *reinterpret_cast<uint2*>(tile + at[k] + 8 * 128) = make_uint2(p[1], p[3]);
+                        }
                         fetch((st + kRound) * kSub + j, cw);
                     }
                     fence_proxy_async();

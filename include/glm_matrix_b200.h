@@ -83,7 +83,7 @@ GLMM_DECLARE_ORTHO(bf16, uint16_t)
  *   codes  [task][target/16][feature/64][lane 0..31][word 0..3] (32-bit words):
  *          a 16 x 64 block of codes in the order in which the lanes of a warp
  *          feed them to the tensor core.  Word s of lane 4g + c holds features
- *          f = 16c + 4s .. f + 3 of targets g and g + 8, each code as q + 8 in
+ *          f = 16s + 4c .. f + 3 of targets g and g + 8, each code as q + 8 in
  *          four bits; from bit 0 up: (g, f), (g+8, f), (g, f+2), (g+8, f+2),
  *          and from bit 16 up the same of f + 1 and f + 3;
  *   scales [task][target/16][group][target%8][target/8%2].
