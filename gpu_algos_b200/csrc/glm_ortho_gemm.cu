@@ -275,9 +275,9 @@ __global__ void __launch_bounds__(kThreads, 1)
                 const uint32_t right0 = desc_address(saddr(sm.stage[0]) + 2 * kPlaneBytes, kSym ? 16 : kPlaneBytes);
                 for (int kb = 0; kb < nkb; ++kb) {
                     const int s = kb % kStages, buf = kb & 1;
-                    if (kb >= 2 && !mbar_wait(&sm.acce[buf], uint32_t(((kb >> 1) - 1) & 1), failed)) break;
-                    if (!mbar_wait(&sm.full[s], uint32_t((kb / kStages) & 1), failed)) break;
-                    if (PAIR && !mbar_wait(&sm.ready[s], uint32_t((kb / kStages) & 1), failed)) break;
+                    if (kb >= 2 && !mbar_wait_one(&sm.acce[buf], uint32_t(((kb >> 1) - 1) & 1), failed)) break;
+                    if (!mbar_wait_one(&sm.full[s], uint32_t((kb / kStages) & 1), failed)) break;
+                    if (PAIR && !mbar_wait_one(&sm.ready[s], uint32_t((kb / kStages) & 1), failed)) break;
                     tc_fence_after();
                     const uint32_t d = tmem + uint32_t(buf * kBN);
                     // K-major: 16 binary16 = 32 bytes on along the row; 8-row groups 1024 bytes apart.
@@ -303,14 +303,14 @@ __global__ void __launch_bounds__(kThreads, 1)
                 commit<PAIR>(&sm.done, mask);
                 // no CTA leaves while a draining warp's arrival is on its way to it
                 for (int b = 0; b < 2 && b < nkb; ++b)
-                    mbar_wait(&sm.acce[b], uint32_t(((nkb - b + 1) / 2 - 1) & 1), failed);
+                    mbar_wait_one(&sm.acce[b], uint32_t(((nkb - b + 1) / 2 - 1) & 1), failed);
             }
-            mbar_wait(&sm.done, 0, nullptr);
+            mbar_wait_one(&sm.done, 0, nullptr);
         } else if (PAIR && warp == 2 && lane == 0 && rank != lead) {
             // tells the even CTA that this CTA's copies of a stage have landed
             for (int kb = 0; kb < nkb; ++kb) {
                 const int s = kb % kStages;
-                if (!mbar_wait(&sm.full[s], uint32_t((kb / kStages) & 1), failed)) break;
+                if (!mbar_wait_one(&sm.full[s], uint32_t((kb / kStages) & 1), failed)) break;
                 fence_proxy_async();
                 mbar_arrive_rank(&sm.ready[s], lead);
             }

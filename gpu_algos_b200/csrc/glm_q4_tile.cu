@@ -185,13 +185,13 @@ __global__ void __launch_bounds__(kThreads, 1)
                 bool ok = true;
                 for (int st = 0; st < nst && ok; ++st) {
                     const int s = st % kStages;
-                    if (!(ok = mbar_wait(&sm.ready[s], uint32_t((st / kStages) & 1), failed))) break;
+                    if (!(ok = mbar_wait_one(&sm.ready[s], uint32_t((st / kStages) & 1), failed))) break;
 #pragma unroll
                     for (int j = 0; j < kSub; ++j) {
                         const int kb = st * kSub + j, grp = kb >> a.group_shift, buf = grp & 1;
                         const bool first = (kb & (gb - 1)) == 0;
                         if (first && grp >= 2 &&
-                            !(ok = mbar_wait(&sm.acce[buf], uint32_t(((grp >> 1) - 1) & 1), failed)))
+                            !(ok = mbar_wait_one(&sm.acce[buf], uint32_t(((grp >> 1) - 1) & 1), failed)))
                             break;
                         tc_fence_after();
                         // K-major: 16 features = 32 bytes on along the row; 8-row groups 1024 bytes apart
@@ -215,14 +215,14 @@ __global__ void __launch_bounds__(kThreads, 1)
                 // no CTA leaves while a draining warp's arrival is on its way to it
                 const int ngrp = nkb >> a.group_shift;
                 for (int b = 0; b < 2 && b < ngrp; ++b)
-                    mbar_wait(&sm.acce[b], uint32_t(((ngrp - b + 1) / 2 - 1) & 1), failed);
+                    mbar_wait_one(&sm.acce[b], uint32_t(((ngrp - b + 1) / 2 - 1) & 1), failed);
             }
-            mbar_wait(&sm.done, 0, nullptr);
+            mbar_wait_one(&sm.done, 0, nullptr);
         } else if (warp == 2 && lane == 0) {
             // tells the even CTA that this CTA's copies of a stage have landed
             for (int st = 0; st < nst; ++st) {
                 const int s = st % kStages;
-                if (!mbar_wait(&sm.xfull[s], uint32_t((st / kStages) & 1), failed)) break;
+                if (!mbar_wait_one(&sm.xfull[s], uint32_t((st / kStages) & 1), failed)) break;
                 fence_proxy_async();
                 mbar_arrive_rank(&sm.ready[s], lead);
             }

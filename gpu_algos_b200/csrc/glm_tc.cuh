@@ -66,6 +66,12 @@ __device__ __forceinline__ bool mbar_wait(unsigned long long* b, uint32_t parity
     return true;
 }
 
+// The same for a role that one thread plays, on whose path every instruction lies: the clock is read only when
+// the barrier is not there yet.
+__device__ __forceinline__ bool mbar_wait_one(unsigned long long* b, uint32_t parity, volatile int* failed) {
+    return mbar_test(b, parity) || mbar_wait(b, parity, failed);
+}
+
 // The same for a whole warp, which comes out of it converged (what follows -- TMEM loads, an arrival for the
 // warp -- needs that) and of one mind.
 __device__ __forceinline__ bool mbar_wait_warp(unsigned long long* b, uint32_t parity, volatile int* failed) {
