@@ -137,6 +137,33 @@ __device__ __forceinline__ void store_split8(__half* hi, int64_t plane, const fl
     *reinterpret_cast<uint4*>(hi + plane) = l;
 }
 
+// Four elements of a row, or as many as are left of it; `whole`: one access.
+template <typename T>
+__device__ __forceinline__ float4 load4(const T* p, int64_t left, bool whole) {
+    alignas(16) T t[4] = {};
+    if (whole) {
+        if constexpr (sizeof(T) == 4) *reinterpret_cast<uint4*>(t) = *reinterpret_cast<const uint4*>(p);
+        else *reinterpret_cast<uint2*>(t) = *reinterpret_cast<const uint2*>(p);
+    } else {
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+            if (i < left) t[i] = p[i];
+    }
+    return make_float4(to_arith<float>(t[0]), to_arith<float>(t[1]), to_arith<float>(t[2]), to_arith<float>(t[3]));
+}
+template <typename T>
+__device__ __forceinline__ void store4(T* p, int64_t left, bool whole, float4 v) {
+    alignas(16) T t[4] = {from_arith<T>(v.x), from_arith<T>(v.y), from_arith<T>(v.z), from_arith<T>(v.w)};
+    if (whole) {
+        if constexpr (sizeof(T) == 4) *reinterpret_cast<uint4*>(p) = *reinterpret_cast<const uint4*>(t);
+        else *reinterpret_cast<uint2*>(p) = *reinterpret_cast<const uint2*>(t);
+    } else {
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+            if (i < left) p[i] = t[i];
+    }
+}
+
 // kGram: D = A = X X^T and D2 = C = bI + cA;  kPoly: D = B = aI + A C;  kApply: D = B X;  kLast: out from B X.
 enum : int { kGram, kPoly, kApply, kLast };
 
@@ -154,6 +181,7 @@ struct GemmArgs {
     int64_t ld;
     void* out;          // kLast
     bool tall, update;
+    bool whole;         // rows of `out` are whole pieces of four elements
     float keep, rate;
     int* status;
 };
@@ -365,55 +393,89 @@ __global__ void __launch_bounds__(kThreads, 1)
             bad = *static_cast<volatile int*>(a.status) != 0;
             for (int p = 0; p < csize; ++p) bad |= ld_cluster_s32(&sm.failed, p) != 0;
         }
-        // Sum over the shares of K in rank order, scale, write; four columns to a thread.  The loops here are
-        // kept rolled: this code runs once per tile, and straight-line code costs an instruction fetch from L2
-        // every eight instructions.
+        // Four columns to a thread, every kRowsAtOnce-th row.  The loops here are kept rolled: this code runs once
+        // per tile, and straight-line code costs an instruction fetch from L2 every eight instructions.
         const int dt = threadIdx.x - kDrainWarp0 * 32;
         constexpr int kRowsAtOnce = kDrainThreads * 4 / kBN;
-        const int c = 4 * (dt % (kBN / 4)), col = n0 + c;
-#pragma unroll 2
-        for (int r = r0 + dt / (kBN / 4); r < r0 + share; r += kRowsAtOnce) {
-            const int row = m0 + r;
-            float4 v;
-            if (a.splits == 1) {
-                v = *reinterpret_cast<const float4*>(tile + r * kTileLd + c);
-            } else {
-                const uint32_t at = saddr(tile + r * kTileLd + c);
-                float4 q[kMaxSplits];
+        const int c = 4 * (dt % (kBN / 4)), col = n0 + c, rt = r0 + dt / (kBN / 4);
+        // The peers' partial sums onto this CTA's own, from the next rank on and around; eight loads in flight.
+        constexpr int kTogether = 8;
+#pragma unroll 1
+        for (int p = 1; p < a.splits; ++p) {
+            const uint32_t peer = (part + uint32_t(p)) & uint32_t(a.splits - 1);
+            const uint32_t from = mapa(saddr(tile + rt * kTileLd + c), PAIR ? 2 * peer + half : peer);
+#pragma unroll 1
+            for (int r = 0; r < share; r += kTogether * kRowsAtOnce) {
+                float4 q[kTogether];
 #pragma unroll
-                for (int p = 0; p < kMaxSplits; ++p)
-                    if (p < a.splits) q[p] = ld_cluster_f4(mapa(at, PAIR ? 2 * p + half : p));
-                v = q[0];
+                for (int j = 0; j < kTogether; ++j)
+                    if (r + j * kRowsAtOnce < share)
+                        q[j] = ld_cluster_f4(from + uint32_t((r + j * kRowsAtOnce) * kTileLd * 4));
 #pragma unroll
-                for (int p = 1; p < kMaxSplits; ++p)
-                    if (p < a.splits) {
-                        v.x += q[p].x;
-                        v.y += q[p].y;
-                        v.z += q[p].z;
-                        v.w += q[p].w;
+                for (int j = 0; j < kTogether; ++j)
+                    if (r + j * kRowsAtOnce < share) {
+                        float4* const at = reinterpret_cast<float4*>(tile + (rt + r + j * kRowsAtOnce) * kTileLd + c);
+                        const float4 v = *at;
+                        *at = make_float4(v.x + q[j].x, v.y + q[j].y, v.z + q[j].z, v.w + q[j].w);
                     }
             }
-            v.x = fmaf(v.x, a.scale, KIND == kPoly && row == col ? a.diag : 0.0f);
-            v.y = fmaf(v.y, a.scale, KIND == kPoly && row == col + 1 ? a.diag : 0.0f);
-            v.z = fmaf(v.z, a.scale, KIND == kPoly && row == col + 2 ? a.diag : 0.0f);
-            v.w = fmaf(v.w, a.scale, KIND == kPoly && row == col + 3 ? a.diag : 0.0f);
-            if constexpr (KIND != kLast) {
-                if (row < a.m && col < a.ld) {
-                    const int64_t at = (task * 2 * a.m + row) * a.ld + col;
-                    store_split4(a.D + at, a.m * a.ld, v);
-                    if constexpr (KIND == kGram) {
-                        const float4 w = make_float4(
-                            fmaf(v.x, a.scale2, row == col ? a.diag : 0.0f),
-                            fmaf(v.y, a.scale2, row == col + 1 ? a.diag : 0.0f),
-                            fmaf(v.z, a.scale2, row == col + 2 ? a.diag : 0.0f),
-                            fmaf(v.w, a.scale2, row == col + 3 ? a.diag : 0.0f));
-                        store_split4(a.D2 + at, a.m * a.ld, w);
+        }
+        // the operator's own arithmetic, in place, and the output as the rows lie
+        T* const out = KIND == kLast ? static_cast<T*>(a.out) + task * a.m * a.n : nullptr;
+        constexpr int kUnroll = KIND == kLast ? 4 : 2;
+#pragma unroll 1
+        for (int rr = rt; rr < r0 + share; rr += kUnroll * kRowsAtOnce) {
+            [[maybe_unused]] float4 old[kUnroll];
+            if constexpr (KIND == kLast) {
+                if (a.update && !a.tall) {
+#pragma unroll
+                    for (int j = 0; j < kUnroll; ++j) {
+                        const int row = m0 + rr + j * kRowsAtOnce;
+                        if (row < a.m && col < a.n) old[j] = load4(out + int64_t(row) * a.n + col, a.n - col, a.whole);
                     }
                 }
             }
-            if (KIND == kLast || mirror) *reinterpret_cast<float4*>(tile + r * kTileLd + c) = v;
+#pragma unroll
+            for (int j = 0; j < kUnroll; ++j) {
+                const int r = rr + j * kRowsAtOnce, row = m0 + r;
+                if (r >= r0 + share) break;
+                float4 v = *reinterpret_cast<const float4*>(tile + r * kTileLd + c);
+                v.x = fmaf(v.x, a.scale, KIND == kPoly && row == col ? a.diag : 0.0f);
+                v.y = fmaf(v.y, a.scale, KIND == kPoly && row == col + 1 ? a.diag : 0.0f);
+                v.z = fmaf(v.z, a.scale, KIND == kPoly && row == col + 2 ? a.diag : 0.0f);
+                v.w = fmaf(v.w, a.scale, KIND == kPoly && row == col + 3 ? a.diag : 0.0f);
+                if constexpr (KIND == kLast) {
+                    if (a.tall) {
+                        *reinterpret_cast<float4*>(tile + r * kTileLd + c) = v;
+                    } else if (row < a.m && col < a.n) {
+                        if (a.update) {
+                            v.x = fmaf(-a.rate, v.x, a.keep * old[j].x);
+                            v.y = fmaf(-a.rate, v.y, a.keep * old[j].y);
+                            v.z = fmaf(-a.rate, v.z, a.keep * old[j].z);
+                            v.w = fmaf(-a.rate, v.w, a.keep * old[j].w);
+                        }
+                        if (bad) v.x = v.y = v.z = v.w = __int_as_float(0x7fc00000);
+                        store4(out + int64_t(row) * a.n + col, a.n - col, a.whole, v);
+                    }
+                } else {
+                    if (row < a.m && col < a.ld) {
+                        const int64_t at = (task * 2 * a.m + row) * a.ld + col;
+                        store_split4(a.D + at, a.m * a.ld, v);
+                        if constexpr (KIND == kGram) {
+                            const float4 w = make_float4(
+                                fmaf(v.x, a.scale2, row == col ? a.diag : 0.0f),
+                                fmaf(v.y, a.scale2, row == col + 1 ? a.diag : 0.0f),
+                                fmaf(v.z, a.scale2, row == col + 2 ? a.diag : 0.0f),
+                                fmaf(v.w, a.scale2, row == col + 3 ? a.diag : 0.0f));
+                            store_split4(a.D2 + at, a.m * a.ld, w);
+                        }
+                    }
+                    if (mirror) *reinterpret_cast<float4*>(tile + r * kTileLd + c) = v;
+                }
+            }
         }
-        if (KIND == kLast || mirror) drain_sync();
+        const bool across = KIND == kLast ? a.tall : mirror;  // the tile is needed column by column too
+        if (across) drain_sync();
         if constexpr (kSym) {
             if (mirror) {
                 // eight rows of one column to a thread: 16 bytes of a row of the mirror image
@@ -436,30 +498,30 @@ __global__ void __launch_bounds__(kThreads, 1)
             }
         }
         if constexpr (KIND == kLast) {
-            T* out = static_cast<T*>(a.out) + task * a.m * a.n;
-            const int share_log2 = 31 - __clz(share);
-            constexpr int kAhead = 8;  // share * kBN is a multiple of 8 * kDrainThreads
+            if (a.tall) {
+                const int share_log2 = 31 - __clz(share);
+                constexpr int kAhead = 8;  // share * kBN is a multiple of 8 * kDrainThreads
 #pragma unroll 1
-            for (int i0 = dt; i0 < share * kBN; i0 += kAhead * kDrainThreads) {
-                int64_t at[kAhead];
-                float v[kAhead], old[kAhead];
+                for (int i0 = dt; i0 < share * kBN; i0 += kAhead * kDrainThreads) {
+                    float old[kAhead];
+                    if (a.update) {
 #pragma unroll
-                for (int j = 0; j < kAhead; ++j) {
-                    // neighbouring threads on neighbouring elements of the output
-                    const int i = i0 + j * kDrainThreads;
-                    const int r = r0 + (a.tall ? i & (share - 1) : i / kBN), c = a.tall ? i >> share_log2 : i % kBN;
-                    const int64_t row = m0 + r, col = n0 + c;
-                    const bool in = row < a.m && col < a.n;
-                    at[j] = !in ? -1 : a.tall ? col * a.m + row : row * a.n + col;
-                    v[j] = tile[r * kTileLd + c];
-                    old[j] = a.update && in ? to_arith<float>(out[at[j]]) : 0.0f;
-                }
+                        for (int j = 0; j < kAhead; ++j) {
+                            const int i = i0 + j * kDrainThreads;
+                            const int64_t row = m0 + r0 + (i & (share - 1)), col = n0 + (i >> share_log2);
+                            old[j] = row < a.m && col < a.n ? to_arith<float>(out[col * a.m + row]) : 0.0f;
+                        }
+                    }
 #pragma unroll
-                for (int j = 0; j < kAhead; ++j) {
-                    if (at[j] < 0) continue;
-                    if (a.update) v[j] = fmaf(-a.rate, v[j], a.keep * old[j]);
-                    if (bad) v[j] = __int_as_float(0x7fc00000);
-                    out[at[j]] = from_arith<T>(v[j]);
+                    for (int j = 0; j < kAhead; ++j) {
+                        // neighbouring threads on neighbouring rows, which lie side by side in the output
+                        const int i = i0 + j * kDrainThreads, r = r0 + (i & (share - 1)), c = i >> share_log2;
+                        const int64_t row = m0 + r, col = n0 + c;
+                        if (row >= a.m || col >= a.n) continue;
+                        float v = tile[r * kTileLd + c];
+                        if (a.update) v = fmaf(-a.rate, v, a.keep * old[j]);
+                        out[col * a.m + row] = from_arith<T>(bad ? __int_as_float(0x7fc00000) : v);
+                    }
                 }
             }
         }
@@ -621,6 +683,7 @@ int ortho_products(const OrthoPlanes& p, const OrthoSteps& steps, T* out, bool t
             g.scale = 1.0f / (sb * sx);
             g.out = out;
             g.tall = tall;
+            g.whole = n % 4 == 0 && (reinterpret_cast<uintptr_t>(out) & (4 * sizeof(T) - 1)) == 0;
             g.update = up != nullptr;
             if (up != nullptr) {
                 g.keep = up->keep;

@@ -94,6 +94,14 @@ __device__ __forceinline__ void tma_load_4d(void* dst, const CUtensorMap* map, i
         : "memory");
 }
 
+// a += s x, b += s y in one instruction
+__device__ __forceinline__ void fma_pair(float& a, float& b, float s, float x, float y) {
+    asm("{\n\t.reg .b64 p, q, r;\n\tmov.b64 p, {%0, %1};\n\tmov.b64 q, {%2, %2};\n\tmov.b64 r, {%3, %4};\n\t"
+        "fma.rn.f32x2 p, q, r, p;\n\tmov.b64 {%0, %1}, p;\n\t}"
+        : "+f"(a), "+f"(b)
+        : "f"(s), "f"(x), "f"(y));
+}
+
 struct TileArgs {
     int64_t nt, ntasks, nobs;
     int64_t nrb;
@@ -249,13 +257,18 @@ __global__ void __launch_bounds__(kThreads, 1)
             if (live && grp + 1 < ngrp) next = *sc;
             if (!(ok = mbar_wait_warp(&sm.accf[buf], uint32_t((grp >> 1) & 1), failed))) break;
             tc_fence_after();
+            // the next sixteen columns load while these are added
+            uint32_t r[2][16];
+            tmem_ld16(tbase + uint32_t(buf * N), r[0]);
+            tmem_wait_ld(r[0]);
 #pragma unroll
             for (int h = 0; h < kCols / 16; ++h) {
-                uint32_t r[16];
-                tmem_ld16(tbase + uint32_t(buf * N + 16 * h), r);
-                tmem_wait_ld(r);
+                if (h + 1 < kCols / 16) tmem_ld16(tbase + uint32_t(buf * N + 16 * (h + 1)), r[(h + 1) & 1]);
 #pragma unroll
-                for (int i = 0; i < 16; ++i) sum[16 * h + i] = fmaf(s, __uint_as_float(r[i]), sum[16 * h + i]);
+                for (int i = 0; i < 16; i += 2)
+                    fma_pair(sum[16 * h + i], sum[16 * h + i + 1], s, __uint_as_float(r[h & 1][i]),
+                             __uint_as_float(r[h & 1][i + 1]));
+                if (h + 1 < kCols / 16) tmem_wait_ld(r[(h + 1) & 1]);
             }
             tc_fence_before();
             __syncwarp();
