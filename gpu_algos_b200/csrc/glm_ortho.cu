@@ -22,10 +22,13 @@ constexpr int kThreads = 256;
 template <typename T>
 __global__ void __launch_bounds__(kThreads)
     ortho_norm_kernel(const T* __restrict__ G, float* __restrict__ V, double* __restrict__ part,
-                      int* __restrict__ status, int64_t size, OrthoUpdate up) {
+                      int* __restrict__ status, int* __restrict__ arrived, int narrived, int64_t size, OrthoUpdate up) {
     __shared__ double red[kThreads / 32];
     pdl_allow_dependents();
-    if (blockIdx.x == 0 && blockIdx.y == 0 && threadIdx.x == 0) *status = 0;
+    if (blockIdx.x == 0 && blockIdx.y == 0) {
+        if (threadIdx.x == 0) *status = 0;
+        for (int i = threadIdx.x; i < narrived; i += kThreads) arrived[i] = 0;
+    }
     const int64_t base = int64_t(blockIdx.y) * size;
     const int64_t stride = int64_t(gridDim.x) * kThreads;
     double s = 0.0;
@@ -164,7 +167,7 @@ template <typename T>
 size_t ortho_workspace(int64_t nf, int64_t nt, int64_t ntasks) {
     const int64_t m = std::min(nf, nt), n = std::max(nf, nt);
     if (m <= kOrthoSmallRows) return 0;
-    return 256 + round_up(size_t(ntasks) * norm_blocks(m * n, ntasks) * 8, 256) +
+    return 256 + round_up(ortho_partial_bytes(m, n, ntasks), 256) + round_up(ortho_arrived_bytes(), 256) + round_up(size_t(ntasks) * norm_blocks(m * n, ntasks) * 8, 256) +
            2 * round_up(size_t(ntasks) * m * padded(n) * 4, 256) + 3 * round_up(size_t(ntasks) * m * padded(m) * 4, 256);
 }
 
@@ -186,17 +189,20 @@ int ortho_run(const T* G, float* V, T* out, int64_t nf, int64_t nt, int64_t ntas
         w += round_up(bytes, 256);
         return p;
     };
-    OrthoPlanes p{m, n, padded(m), padded(n), ntasks, {}, nullptr, nullptr, nullptr};
+    OrthoPlanes p{m, n, padded(m), padded(n), ntasks, {}, nullptr, nullptr, nullptr, nullptr, nullptr};
     int* status = reinterpret_cast<int*>(take(4));
     const int64_t nb = norm_blocks(size, ntasks);
     double* part = reinterpret_cast<double*>(take(size_t(ntasks) * nb * 8));
+    p.partial = reinterpret_cast<float4*>(take(ortho_partial_bytes(m, n, ntasks)));
+    p.arrived = reinterpret_cast<int*>(take(ortho_arrived_bytes()));
     for (__half*& x : p.X) x = reinterpret_cast<__half*>(take(size_t(ntasks) * m * p.ld_n * 4));
     p.A = reinterpret_cast<__half*>(take(size_t(ntasks) * m * p.ld_m * 4));
     p.B = reinterpret_cast<__half*>(take(size_t(ntasks) * m * p.ld_m * 4));
     p.C = reinterpret_cast<__half*>(take(size_t(ntasks) * m * p.ld_m * 4));
     const OrthoUpdate up = update != nullptr ? *update : OrthoUpdate{};
     set_last_path("ortho_tensor");
-    ortho_norm_kernel<T><<<dim3(unsigned(nb), unsigned(ntasks)), kThreads, 0, stream>>>(G, V, part, status, size, up);
+    ortho_norm_kernel<T><<<dim3(unsigned(nb), unsigned(ntasks)), kThreads, 0, stream>>>(
+        G, V, part, status, p.arrived, int(ortho_arrived_bytes() / sizeof(int)), size, up);
     count_launch();
     int st = launch_status();
     if (st != GLMB_OK) return st;

@@ -36,7 +36,11 @@ struct OrthoPlanes {
     __half* A;     // m x m
     __half* B;
     __half* C;
+    float4* partial;  // ortho_partial_bytes(): sums of tiles whose K two clusters share (nullptr for none)
+    int* arrived;     // ortho_arrived_bytes(), zero
 };
+size_t ortho_partial_bytes(int64_t m, int64_t n, int64_t ntasks);
+size_t ortho_arrived_bytes();
 // The power of two that X's planes carry before a step.
 float ortho_x_scale(const OrthoStep& s);
 // All steps from X[0] (scaled by ortho_x_scale of the first) to `out` or, with `up`, the model's update;

@@ -41,6 +41,7 @@ constexpr int kStages = 3;
 constexpr int kPlaneBytes = 128 * kBK * 2;  // 128 rows (or columns) of one plane: 16 KB
 constexpr int kStageBytes = 4 * kPlaneBytes;  // left hi, lo, right hi, lo
 constexpr int kMaxSplits = 8;
+constexpr int64_t kMaxHalved = 74;  // CTAs of tiles that may be halved: beyond, whole tiles fill the SMs
 constexpr int kDrainWarp0 = 4, kDrainWarps = 8, kDrainThreads = kDrainWarps * 32;
 constexpr int kThreads = (kDrainWarp0 + kDrainWarps) * 32;
 // 384 threads launch with 168 registers each; the control warpgroup gives its share to the two that drain
@@ -57,6 +58,7 @@ struct GemmSmem {
     unsigned long long done;
     uint32_t tmem_base;
     int failed;
+    int turn;
 };
 
 // D (f32) from binary16 A and B; K-major A, B K- or MN-major.
@@ -173,6 +175,9 @@ struct GemmArgs {
     int32_t units;      // tiles a task has
     int32_t nkb;        // 64-deep blocks of K
     int32_t splits;     // CTAs (pairs) of a cluster, each with its share of K
+    int32_t halves;     // 2: two clusters work on a tile, each with half of K (splits is 1 then)
+    float4* partial;    // halves == 2: sums of the half that is done first, [tile, CTA of the pair][column / 4][thread]
+    int* arrived;       // [tile, CTA of the pair], zero between launches
     float scale;        // of the accumulated sum
     float scale2;       // kGram: of D on its way to D2
     float diag;         // on the diagonal of D2 (kGram) or D (kPoly)
@@ -208,7 +213,8 @@ __global__ void __launch_bounds__(kThreads, 1)
     const uint32_t lead = PAIR ? (rank & ~1u) : rank;     // the CTA that issues the MMAs
     const int csize = a.splits * (PAIR ? 2 : 1);
 
-    const int64_t cluster = blockIdx.x / csize;
+    const int64_t cluster = blockIdx.x / csize / a.halves;
+    const int share_of = a.halves == 1 ? int(part) : int(blockIdx.x / csize % 2), shares = a.splits * a.halves;
     const int64_t task = cluster / a.units;
     const int u = int(cluster % a.units);
     int ti, tj;
@@ -229,7 +235,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     const int n0 = tj * kBN;
     const int nb0 = n0 + int(half) * 128;            // the columns this CTA stages
     // this CTA's share of K
-    const int kb0 = int(int64_t(a.nkb) * part / a.splits), kb1 = int(int64_t(a.nkb) * (part + 1) / a.splits);
+    const int kb0 = int(int64_t(a.nkb) * share_of / shares), kb1 = int(int64_t(a.nkb) * (share_of + 1) / shares);
     const int nkb = kb1 - kb0;
 
     if (tid == 0) {
@@ -269,6 +275,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     const uint32_t tmem = sm.tmem_base;
     volatile int* failed = &sm.failed;
     float* tile = reinterpret_cast<float*>(sm.stage[0]);
+    bool finish = true;  // this CTA has (its rows of) the whole sum
     pdl_allow_dependents();
     pdl_wait_for_producer();
 
@@ -371,8 +378,41 @@ __global__ void __launch_bounds__(kThreads, 1)
             __syncwarp();
             if (lane == 0) mbar_arrive_rank(&sm.acce[buf], lead);
         }
+        if (a.halves == 2) {
+            // Both halves leave their sums in global memory; the one that is there last (nobody waits) adds the
+            // other's to its own -- two summands, so the order does not matter -- and goes on alone.
+            if (!ok) {
+#pragma unroll
+                for (int i = 0; i < kCols; ++i) sum[i] = __int_as_float(0x7fc00000);
+                ok = true;
+            }
+            const int64_t which = cluster * (PAIR ? 2 : 1) + half;
+            const int dt = threadIdx.x - kDrainWarp0 * 32;
+            float4* const slot = a.partial + which * 2 * (kCols / 4) * kDrainThreads + dt;
+#pragma unroll
+            for (int i = 0; i < kCols; i += 4)
+                slot[(share_of * (kCols / 4) + i / 4) * kDrainThreads] =
+                    make_float4(sum[i], sum[i + 1], sum[i + 2], sum[i + 3]);
+            __threadfence();
+            drain_sync();
+            if (dt == 0) sm.turn = atomicAdd(&a.arrived[which], 1);
+            drain_sync();
+            finish = sm.turn == 1;
+            if (finish) {
+                if (dt == 0) a.arrived[which] = 0;  // for the next launch
+                __threadfence();
+#pragma unroll
+                for (int i = 0; i < kCols; i += 4) {
+                    const float4 v = __ldcg(slot + ((share_of ^ 1) * (kCols / 4) + i / 4) * kDrainThreads);
+                    sum[i] += v.x;
+                    sum[i + 1] += v.y;
+                    sum[i + 2] += v.z;
+                    sum[i + 3] += v.w;
+                }
+            }
+        }
         // every copy has landed and every MMA of this CTA's stages has retired: the stages become the tile
-        if (ok) {
+        if (ok && finish) {
             float* row = tile + (32 * quarter + lane) * kTileLd + side * kCols;
 #pragma unroll
             for (int i = 0; i < kCols; i += 4)
@@ -384,7 +424,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     __syncthreads();
     if (csize > 1) cluster_sync();  // the peers' partial tiles are complete
 
-    if (warp >= kDrainWarp0) {
+    if (warp >= kDrainWarp0 && finish) {
         const int share = kBM / a.splits;  // rows of the tile this CTA finishes
         const int r0 = int(part) * share;
         const bool mirror = kSym && ti != tj;
@@ -556,31 +596,67 @@ bool plane_map(CUtensorMap* map, const __half* base, int64_t cols, int64_t rows,
 // How a product is cut: the shape of its tiles and the shares of K.
 struct Cut {
     bool pair;
-    int splits;
+    int splits, halves;
     int64_t tiles_m, tiles_n, units;
 };
 
+// Clusters of `csize` CTAs, one to an SM, that the device holds at once: the SMs of a GPC come in numbers that
+// larger clusters do not divide (148 SMs hold 74 clusters of 2, 33 of 4 and 15 of 8).
+int64_t clusters_at_once(int csize) {
+    static std::atomic<int> known[64][4];
+    int dev = 0, log2 = csize == 1 ? 0 : csize == 2 ? 1 : csize == 4 ? 2 : 3;
+    if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= 64) return std::max(1, sm_count() / csize);
+    int n = known[dev][log2].load(std::memory_order_relaxed);
+    if (n == 0) {
+        auto kernel = ortho_gemm_kernel<false, kGram, float>;
+        static std::atomic<uint64_t> attr{0};
+        const size_t smem = sizeof(GemmSmem) + 1024;
+        cudaLaunchConfig_t cfg = {};
+        cfg.gridDim = dim3(unsigned(csize));
+        cfg.blockDim = dim3(kThreads);
+        cfg.dynamicSmemBytes = smem;
+        cudaLaunchAttribute at[1];
+        at[0].id = cudaLaunchAttributeClusterDimension;
+        at[0].val.clusterDim.x = unsigned(csize);
+        at[0].val.clusterDim.y = at[0].val.clusterDim.z = 1;
+        cfg.attrs = at;
+        cfg.numAttrs = 1;
+        if (set_smem_limit_once(attr, kernel, smem) != cudaSuccess ||
+            cudaOccupancyMaxActiveClusters(&n, kernel, &cfg) != cudaSuccess || n <= 0) {
+            (void)cudaGetLastError();
+            n = std::max(1, sm_count() / csize * 7 / 8);
+        }
+        known[dev][log2].store(n, std::memory_order_relaxed);
+    }
+    return n;
+}
+
 // The cut with the least estimated time, in clocks: waves of clusters over the
 // SMs times (blocks of K per share + what a tile costs besides).  A pair's
-// block takes its 12 MMAs of 128 clocks; a single CTA's 12 MMAs of 64 wait for
-// the same bytes, about 1000 clocks.
+// block is its 12 MMAs of 128 clocks; a single CTA's 12 MMAs of half that
+// size take hardly less (1390 measured).
 Cut cut_product(int64_t m, int64_t n, int64_t nkb, int64_t ntasks, bool sym) {
     Cut best{};
     double least = 0.0;
     for (const bool pair : {true, false}) {
         const int64_t bt = pair ? 256 : 128, tm = (m + bt - 1) / bt, tn = (n + bt - 1) / bt;
         const int64_t units = sym ? tm * (tm + 1) / 2 : tm * tn;
-        for (int splits = 1; splits <= (pair ? kMaxSplits / 2 : kMaxSplits); splits *= 2) {
-            if (splits > 1 && nkb < 2 * splits) break;
-            const int csize = splits * (pair ? 2 : 1);
-            const int64_t at_once = std::max<int64_t>(1, sm_count() / csize);
-            const int64_t waves = (units * ntasks + at_once - 1) / at_once;
-            const double block = pair ? 1600.0 : 1000.0;
-            const double tile = 3000.0 + (pair ? 5000.0 : 2500.0) / splits + (splits > 1 ? 2500.0 : 0.0);
-            const double t = double(waves) * (double((nkb + splits - 1) / splits) * block + tile);
-            if (least == 0.0 || t < least) {
-                least = t;
-                best = Cut{pair, splits, tm, tn, units};
+        for (int shares = 1; shares <= (pair ? kMaxSplits / 2 : kMaxSplits); shares *= 2) {
+            if (shares > 1 && nkb < 2 * shares) break;
+            for (int halves = 1; halves <= 2; ++halves) {
+                // two halves of a tile meet in global memory: only for few tiles, whose partial sums stay small
+                if (halves == 2 && (shares != 2 || units * ntasks * (pair ? 2 : 1) > kMaxHalved)) continue;
+                const int splits = shares / halves;
+                const int64_t at_once = clusters_at_once(splits * (pair ? 2 : 1));
+                const int64_t waves = (units * ntasks * halves + at_once - 1) / at_once;
+                const double block = pair ? 1550.0 : 1390.0;
+                const double tile = 4500.0 + (pair ? 10000.0 : 5000.0) / splits + (splits > 1 ? 2500.0 : 0.0) +
+                                    (halves > 1 ? (pair ? 5000.0 : 2500.0) : 0.0);
+                const double t = double(waves) * (double((nkb + shares - 1) / shares) * block + tile);
+                if (least == 0.0 || t < least) {
+                    least = t;
+                    best = Cut{pair, splits, halves, tm, tn, units};
+                }
             }
         }
     }
@@ -597,7 +673,7 @@ cudaError_t launch_gemm(const CUtensorMap& left, const CUtensorMap& right, const
     if (e != cudaSuccess) return e;
     const int csize = args.splits * (PAIR ? 2 : 1);
     cudaLaunchConfig_t cfg = {};
-    cfg.gridDim = dim3(unsigned(int64_t(args.units) * ntasks * csize));
+    cfg.gridDim = dim3(unsigned(int64_t(args.units) * ntasks * csize * args.halves));
     cfg.blockDim = dim3(kThreads);
     cfg.dynamicSmemBytes = smem;
     cfg.stream = stream;
@@ -620,6 +696,7 @@ cudaError_t launch_cut(const Cut& cut, const CUtensorMap& left, const CUtensorMa
     args.tiles_n = int32_t(cut.tiles_n);
     args.units = int32_t(cut.units);
     args.splits = cut.splits;
+    args.halves = cut.halves;
     return cut.pair ? launch_gemm<true, KIND, T>(left, right, args, ntasks, stream)
                     : launch_gemm<false, KIND, T>(left, right, args, ntasks, stream);
 }
@@ -629,6 +706,25 @@ float scale_for(double bound) { return float(std::exp2(15.0 - std::ceil(std::log
 
 }  // namespace
 
+namespace {
+struct Cuts {
+    Cut gram, poly, apply;
+    Cuts(int64_t m, int64_t n, int64_t ntasks)
+        : gram(cut_product(m, m, (n + kBK - 1) / kBK, ntasks, true)),
+          poly(cut_product(m, m, (m + kBK - 1) / kBK, ntasks, true)),
+          apply(cut_product(m, n, (m + kBK - 1) / kBK, ntasks, false)) {}
+};
+}  // namespace
+
+size_t ortho_partial_bytes(int64_t m, int64_t n, int64_t ntasks) {
+    const Cuts cuts(m, n, ntasks);
+    size_t most = 0;
+    for (const Cut& c : {cuts.gram, cuts.poly, cuts.apply})
+        if (c.halves == 2) most = std::max(most, size_t(c.units * ntasks) * 2 * (c.pair ? 2 * 128 * 256 : 128 * 128) * 4);
+    return most;
+}
+size_t ortho_arrived_bytes() { return size_t(kMaxHalved) * sizeof(int); }
+
 float ortho_x_scale(const OrthoStep& s) { return scale_for(s.x_max); }
 
 template <typename T>
@@ -636,8 +732,8 @@ int ortho_products(const OrthoPlanes& p, const OrthoSteps& steps, T* out, bool t
                    cudaStream_t stream) {
     const int64_t m = p.m, n = p.n;
     const int64_t kbn = (n + kBK - 1) / kBK, kbm = (m + kBK - 1) / kBK;
-    const Cut gram = cut_product(m, m, kbn, p.ntasks, true), poly = cut_product(m, m, kbm, p.ntasks, true),
-              apply = cut_product(m, n, kbm, p.ntasks, false);
+    const Cuts cuts(m, n, p.ntasks);
+    const Cut &gram = cuts.gram, &poly = cuts.poly, &apply = cuts.apply;
     for (const Cut& c : {gram, poly, apply})
         if (c.units * p.ntasks > (int64_t(1) << 27)) return GLMB_ERR_TOO_LARGE;
     CUtensorMap x_rows[2], x_cols[2], a_rows, b_rows, c_rows;
@@ -656,6 +752,8 @@ int ortho_products(const OrthoPlanes& p, const OrthoSteps& steps, T* out, bool t
         const bool last = k + 1 == steps.n;
         GemmArgs g{};
         g.status = status;
+        g.partial = p.partial;
+        g.arrived = p.arrived;
         g.m = g.n = m;
         g.nkb = int32_t(kbn);
         g.scale = sa / (sx * sx);
