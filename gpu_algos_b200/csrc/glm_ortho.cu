@@ -66,52 +66,92 @@ __global__ void __launch_bounds__(kThreads)
     }
 }
 
-// 64 x 64 tiles of X = scale * U / |U| into its planes, transposed when the matrix is taller than wide;
-// columns that fill up a row to ld (and rows past m: none) are zero.
+// scale / |U| of a task from its blocks' shares, by the first warp; 0 for a zero matrix.
+__device__ __forceinline__ double inverse_norm(const double* part, int nparts, double scale, double* shared) {
+    if (threadIdx.x < 32) {
+        double ss = 0.0;
+        for (int i = threadIdx.x; i < nparts; i += 32) ss += part[i];
+#pragma unroll
+        for (int off = 16; off > 0; off >>= 1) ss += __shfl_xor_sync(0xffffffffu, ss, off);
+        if (threadIdx.x == 0) *shared = ss == 0.0 ? 0.0 : scale / sqrt(ss);
+    }
+    __syncthreads();
+    return *shared;
+}
+
+// u * inv, in float unless inv leaves float's comfortable range (norms near its ends)
+struct Scaled {
+    double inv;
+    float inv_f;
+    bool wide;
+    __device__ explicit Scaled(double v) : inv(v), inv_f(float(v)), wide(!(v == 0.0 || (v > 1e-30 && v < 1e30))) {}
+    __device__ __forceinline__ float operator()(float u) const {
+        return wide ? float(double(u) * inv) : u * inv_f;
+    }
+};
+
+__device__ __forceinline__ void put_split2(__half* dst, int64_t plane, float a, float b) {
+    const __half2 h = __floats2half2_rn(a, b);
+    const float2 f = __half22float2(h);
+    *reinterpret_cast<__half2*>(dst) = h;
+    *reinterpret_cast<__half2*>(dst + plane) = __floats2half2_rn(a - f.x, b - f.y);
+}
+
+// X = scale * U / |U| into its planes, for matrices at least as wide as tall: two neighbouring columns to a
+// thread, four rows at a time.  Columns that fill up a row to ld are zero.  Bound by HBM.
 template <typename T>
 __global__ void __launch_bounds__(kThreads)
     ortho_split_kernel(const T* __restrict__ G, const float* __restrict__ V, const double* __restrict__ part, int nparts,
-                       __half* __restrict__ X, int64_t m, int64_t n, int64_t ld, bool tall, float scale, OrthoUpdate up) {
-    __shared__ float t[64][65];
-    __shared__ double inv_s;
+                       __half* __restrict__ X, int64_t m, int64_t n, int64_t ld, float scale, OrthoUpdate up) {
+    __shared__ double shared;
     pdl_allow_dependents();
     pdl_wait_for_producer();
     const int64_t task = blockIdx.z, base = task * m * n;
-    if (threadIdx.x < 32) {
-        double ss = 0.0;
-        for (int i = threadIdx.x; i < nparts; i += 32) ss += part[task * nparts + i];
+    const Scaled scaled(inverse_norm(part + task * nparts, nparts, scale, &shared));
+    constexpr int kRows = 4;
+    const int64_t tiles_n = (ld / 2 + kThreads - 1) / kThreads, tiles = tiles_n * ((m + kRows - 1) / kRows);
+    for (int64_t tile = blockIdx.x; tile < tiles; tile += gridDim.x) {
+        const int64_t i0 = tile / tiles_n * kRows, j = (tile % tiles_n * kThreads + threadIdx.x) * 2;
+        if (j >= ld) continue;
+        float u[kRows][2];
 #pragma unroll
-        for (int off = 16; off > 0; off >>= 1) ss += __shfl_xor_sync(0xffffffffu, ss, off);
-        if (threadIdx.x == 0) inv_s = ss == 0.0 ? 0.0 : double(scale) / sqrt(ss);
+        for (int i = 0; i < kRows; ++i)
+#pragma unroll
+            for (int k = 0; k < 2; ++k)
+                u[i][k] = i0 + i < m && j + k < n ? ortho_direction(G, V, base + (i0 + i) * n + j + k, up) : 0.0f;
+#pragma unroll
+        for (int i = 0; i < kRows; ++i)
+            if (i0 + i < m)
+                put_split2(X + (task * 2 * m + i0 + i) * ld + j, m * ld, scaled(u[i][0]), scaled(u[i][1]));
     }
+}
+
+// The same of matrices taller than wide, transposed through 64 x 64 tiles.
+template <typename T>
+__global__ void __launch_bounds__(kThreads)
+    ortho_split_tall_kernel(const T* __restrict__ G, const float* __restrict__ V, const double* __restrict__ part,
+                            int nparts, __half* __restrict__ X, int64_t m, int64_t n, int64_t ld, float scale,
+                            OrthoUpdate up) {
+    __shared__ float t[64][65];
+    __shared__ double shared;
+    pdl_allow_dependents();
+    pdl_wait_for_producer();
+    const int64_t task = blockIdx.z, base = task * m * n;
+    const Scaled scaled(inverse_norm(part + task * nparts, nparts, scale, &shared));
     const int64_t tiles_n = (n + 63) / 64, tiles = tiles_n * ((m + 63) / 64);
-    __syncthreads();
-    const double inv = inv_s;
     for (int64_t tile = blockIdx.x; tile < tiles; tile += gridDim.x) {
         const int64_t i0 = tile / tiles_n * 64, j0 = tile % tiles_n * 64;
-#pragma unroll 4
+#pragma unroll 8
         for (int e = threadIdx.x; e < 64 * 64; e += kThreads) {
             // neighbouring threads on neighbouring elements of the matrix as it lies in memory
-            const int i = tall ? e & 63 : e >> 6, j = tall ? e >> 6 : e & 63;
-            float v = 0.0f;
-            if (i0 + i < m && j0 + j < n) {
-                const int64_t at = base + (tall ? (j0 + j) * m + i0 + i : (i0 + i) * n + j0 + j);
-                v = float(double(ortho_direction(G, V, at, up)) * inv);
-            }
-            t[i][j] = v;
+            const int i = e & 63, j = e >> 6;
+            t[i][j] = i0 + i < m && j0 + j < n ? scaled(ortho_direction(G, V, base + (j0 + j) * m + i0 + i, up)) : 0.0f;
         }
         __syncthreads();
 #pragma unroll 4
         for (int e = threadIdx.x; e < 64 * 32; e += kThreads) {
             const int i = e >> 5, j = 2 * (e & 31);
-            if (i0 + i < m && j0 + j < ld) {
-                const float a = t[i][j], b = t[i][j + 1];
-                const __half2 h = __floats2half2_rn(a, b);
-                const float2 f = __half22float2(h);
-                __half* dst = X + (task * 2 * m + i0 + i) * ld + j0 + j;
-                *reinterpret_cast<__half2*>(dst) = h;
-                *reinterpret_cast<__half2*>(dst + m * ld) = __floats2half2_rn(a - f.x, b - f.y);
-            }
+            if (i0 + i < m && j0 + j < ld) put_split2(X + (task * 2 * m + i0 + i) * ld + j0 + j, m * ld, t[i][j], t[i][j + 1]);
         }
         __syncthreads();
     }
@@ -206,12 +246,14 @@ int ortho_run(const T* G, float* V, T* out, int64_t nf, int64_t nt, int64_t ntas
     count_launch();
     int st = launch_status();
     if (st != GLMB_OK) return st;
-    const int64_t tiles = (n + 63) / 64 * ((m + 63) / 64);
+    const int64_t tiles = tall ? (n + 63) / 64 * ((m + 63) / 64)
+                               : (p.ld_n / 2 + kThreads - 1) / kThreads * ((m + 3) / 4);
     const int64_t most = std::max<int64_t>(1, 8 * int64_t(sm_count()) / ntasks);
     const cudaError_t e =
-        pdl_launch(ortho_split_kernel<T>, dim3(unsigned(std::min(tiles, most)), 1, unsigned(ntasks)), dim3(kThreads), 0,
-                   stream, G, static_cast<const float*>(V), static_cast<const double*>(part), int(nb), p.X[0], m, n,
-                   p.ld_n, tall, ortho_x_scale(steps.step[0]), up);
+        pdl_launch(tall ? ortho_split_tall_kernel<T> : ortho_split_kernel<T>,
+                   dim3(unsigned(std::min(tiles, most)), 1, unsigned(ntasks)), dim3(kThreads), 0, stream, G,
+                   static_cast<const float*>(V), static_cast<const double*>(part), int(nb), p.X[0], m, n, p.ld_n,
+                   ortho_x_scale(steps.step[0]), up);
     count_launch();
     if (e != cudaSuccess) return int(e);
     return ortho_products<T>(p, steps, out, tall, update, status, stream);

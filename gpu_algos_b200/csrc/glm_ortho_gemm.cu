@@ -439,24 +439,27 @@ __global__ void __launch_bounds__(kThreads, 1)
         constexpr int kRowsAtOnce = kDrainThreads * 4 / kBN;
         const int c = 4 * (dt % (kBN / 4)), col = n0 + c, rt = r0 + dt / (kBN / 4);
         // The peers' partial sums onto this CTA's own, from the next rank on and around; eight loads in flight.
-        constexpr int kTogether = 8;
+        if (a.splits > 1) {
+            constexpr int kTogether = 8;
+            const int items_log2 = 31 - __clz(share / kRowsAtOnce), loads = (a.splits - 1) << items_log2;
+            const uint32_t at = saddr(tile + rt * kTileLd + c);
 #pragma unroll 1
-        for (int p = 1; p < a.splits; ++p) {
-            const uint32_t peer = (part + uint32_t(p)) & uint32_t(a.splits - 1);
-            const uint32_t from = mapa(saddr(tile + rt * kTileLd + c), PAIR ? 2 * peer + half : peer);
-#pragma unroll 1
-            for (int r = 0; r < share; r += kTogether * kRowsAtOnce) {
+            for (int i = 0; i < loads; i += kTogether) {
                 float4 q[kTogether];
 #pragma unroll
                 for (int j = 0; j < kTogether; ++j)
-                    if (r + j * kRowsAtOnce < share)
-                        q[j] = ld_cluster_f4(from + uint32_t((r + j * kRowsAtOnce) * kTileLd * 4));
+                    if (i + j < loads) {
+                        const uint32_t peer = (part + 1u + uint32_t((i + j) >> items_log2)) & uint32_t(a.splits - 1);
+                        const int row = ((i + j) & ((1 << items_log2) - 1)) * kRowsAtOnce;
+                        q[j] = ld_cluster_f4(mapa(at + uint32_t(row * kTileLd * 4), PAIR ? 2 * peer + half : peer));
+                    }
 #pragma unroll
                 for (int j = 0; j < kTogether; ++j)
-                    if (r + j * kRowsAtOnce < share) {
-                        float4* const at = reinterpret_cast<float4*>(tile + (rt + r + j * kRowsAtOnce) * kTileLd + c);
-                        const float4 v = *at;
-                        *at = make_float4(v.x + q[j].x, v.y + q[j].y, v.z + q[j].z, v.w + q[j].w);
+                    if (i + j < loads) {
+                        const int row = ((i + j) & ((1 << items_log2) - 1)) * kRowsAtOnce;
+                        float4* const to = reinterpret_cast<float4*>(tile + (rt + row) * kTileLd + c);
+                        const float4 v = *to;
+                        *to = make_float4(v.x + q[j].x, v.y + q[j].y, v.z + q[j].z, v.w + q[j].w);
                     }
             }
         }
