@@ -40,7 +40,7 @@ constexpr int kBK = 64;   // K per stage: 128 bytes of binary16, one swizzle row
 constexpr int kStages = 3;
 constexpr int kPlaneBytes = 128 * kBK * 2;  // 128 rows (or columns) of one plane: 16 KB
 constexpr int kStageBytes = 4 * kPlaneBytes;  // left hi, lo, right hi, lo
-constexpr int kMaxSplits = 8;
+constexpr int kMaxSplits = 16;  // CTAs of a cluster
 constexpr int64_t kMaxHalved = 74;  // CTAs of tiles that may be halved: beyond, whole tiles fill the SMs
 constexpr int kDrainWarp0 = 4, kDrainWarps = 8, kDrainThreads = kDrainWarps * 32;
 constexpr int kThreads = (kDrainWarp0 + kDrainWarps) * 32;
@@ -543,7 +543,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         if constexpr (KIND == kLast) {
             if (a.tall) {
                 const int share_log2 = 31 - __clz(share);
-                constexpr int kAhead = 8;  // share * kBN is a multiple of 8 * kDrainThreads
+                constexpr int kAhead = 4;  // share * kBN is a multiple of 4 * kDrainThreads
 #pragma unroll 1
                 for (int i0 = dt; i0 < share * kBN; i0 += kAhead * kDrainThreads) {
                     float old[kAhead];
@@ -604,11 +604,12 @@ struct Cut {
 };
 
 // Clusters of `csize` CTAs, one to an SM, that the device holds at once: the SMs of a GPC come in numbers that
-// larger clusters do not divide (148 SMs hold 74 clusters of 2, 33 of 4 and 15 of 8).
+// larger clusters do not divide (148 SMs hold 74 clusters of 2, 33 of 4, 15 of 8 and 7 of 16).
 int64_t clusters_at_once(int csize) {
-    static std::atomic<int> known[64][4];
-    int dev = 0, log2 = csize == 1 ? 0 : csize == 2 ? 1 : csize == 4 ? 2 : 3;
-    if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= 64) return std::max(1, sm_count() / csize);
+    static std::atomic<int> known[64][5];
+    int dev = 0, log2 = 0;
+    while ((1 << log2) < csize) ++log2;
+    if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= 64) return csize > 8 ? 0 : std::max(1, sm_count() / csize);
     int n = known[dev][log2].load(std::memory_order_relaxed);
     if (n == 0) {
         auto kernel = ortho_gemm_kernel<false, kGram, float>;
@@ -625,13 +626,14 @@ int64_t clusters_at_once(int csize) {
         cfg.attrs = at;
         cfg.numAttrs = 1;
         if (set_smem_limit_once(attr, kernel, smem) != cudaSuccess ||
+            (csize > 8 && cudaFuncSetAttribute(kernel, cudaFuncAttributeNonPortableClusterSizeAllowed, 1) != cudaSuccess) ||
             cudaOccupancyMaxActiveClusters(&n, kernel, &cfg) != cudaSuccess || n <= 0) {
             (void)cudaGetLastError();
-            n = std::max(1, sm_count() / csize * 7 / 8);
+            n = csize > 8 ? 0 : std::max(1, sm_count() / csize * 7 / 8);
         }
-        known[dev][log2].store(n, std::memory_order_relaxed);
+        known[dev][log2].store(n == 0 ? -1 : n, std::memory_order_relaxed);
     }
-    return n;
+    return std::max(n, 0);
 }
 
 // The cut with the least estimated time, in clocks: waves of clusters over the
@@ -644,13 +646,14 @@ Cut cut_product(int64_t m, int64_t n, int64_t nkb, int64_t ntasks, bool sym) {
     for (const bool pair : {true, false}) {
         const int64_t bt = pair ? 256 : 128, tm = (m + bt - 1) / bt, tn = (n + bt - 1) / bt;
         const int64_t units = sym ? tm * (tm + 1) / 2 : tm * tn;
-        for (int shares = 1; shares <= (pair ? kMaxSplits / 2 : kMaxSplits); shares *= 2) {
+        for (int shares = 1; shares <= (pair ? kMaxSplits / 4 : kMaxSplits); shares *= 2) {
             if (shares > 1 && nkb < 2 * shares) break;
             for (int halves = 1; halves <= 2; ++halves) {
                 // two halves of a tile meet in global memory: only for few tiles, whose partial sums stay small
                 if (halves == 2 && (shares != 2 || units * ntasks * (pair ? 2 : 1) > kMaxHalved)) continue;
                 const int splits = shares / halves;
                 const int64_t at_once = clusters_at_once(splits * (pair ? 2 : 1));
+                if (at_once == 0) continue;
                 const int64_t waves = (units * ntasks * halves + at_once - 1) / at_once;
                 const double block = pair ? 1550.0 : 1390.0;
                 const double tile = 4500.0 + (pair ? 10000.0 : 5000.0) / splits + (splits > 1 ? 2500.0 : 0.0) +
@@ -675,6 +678,16 @@ cudaError_t launch_gemm(const CUtensorMap& left, const CUtensorMap& right, const
     cudaError_t e = set_smem_limit_once(attr, kernel, smem);
     if (e != cudaSuccess) return e;
     const int csize = args.splits * (PAIR ? 2 : 1);
+    if (csize > 8) {
+        static std::atomic<uint64_t> wide{0};
+        int dev = 0;
+        if ((e = cudaGetDevice(&dev)) != cudaSuccess) return e;
+        const uint64_t bit = dev >= 0 && dev < 64 ? uint64_t(1) << dev : 0;
+        if (bit == 0 || (wide.load(std::memory_order_acquire) & bit) == 0) {
+            if ((e = cudaFuncSetAttribute(kernel, cudaFuncAttributeNonPortableClusterSizeAllowed, 1)) != cudaSuccess) return e;
+            wide.fetch_or(bit, std::memory_order_release);
+        }
+    }
     cudaLaunchConfig_t cfg = {};
     cfg.gridDim = dim3(unsigned(int64_t(args.units) * ntasks * csize * args.halves));
     cfg.blockDim = dim3(kThreads);

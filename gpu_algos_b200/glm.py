@@ -20,6 +20,7 @@ on ``stream``.
 from __future__ import annotations
 
 import ctypes
+import functools
 import math
 
 import torch
@@ -393,16 +394,28 @@ class Q4Model:
         _matrix_suffix(dtype)
         if self.group not in (64, 128):
             raise ValueError(f"group is {group}, expected 64 or 128")
-        L = capi.lib()
-        codes = L.glmm_q4_codes_bytes(nf, nt, ntasks)
+        codes, count = _q4_sizes(nf, nt, ntasks, self.group)
         # one allocation; the scales follow the codes, which are a multiple of 512 bytes
-        count = L.glmm_q4_scales_count(nf, nt, ntasks, self.group)
-        held = torch.empty(codes + count * dtype.itemsize, dtype=torch.uint8, device=device)
-        self.codes, self.scales = held[:codes], held[codes:].view(dtype)
+        self._held = torch.empty(codes + count * dtype.itemsize, dtype=torch.uint8, device=device)
+        self._codes_bytes = codes
+        self._codes_ptr = self._held.data_ptr()
+        self._scales_ptr = self._codes_ptr + codes
+        self.device = self._held.device
 
     @property
-    def device(self):
-        return self.codes.device
+    def codes(self):
+        return self._held[:self._codes_bytes]
+
+    @property
+    def scales(self):
+        return self._held[self._codes_bytes:].view(self.dtype)
+
+
+@functools.lru_cache(maxsize=256)
+def _q4_sizes(nf: int, nt: int, ntasks: int, group: int):
+    """Bytes of codes and number of scales, as the library lays them out."""
+    L = capi.lib()
+    return L.glmm_q4_codes_bytes(nf, nt, ntasks), L.glmm_q4_scales_count(nf, nt, ntasks, group)
 
 
 def quantize_q4(M, group: int = 128, out=None, stream=None) -> Q4Model:
@@ -421,7 +434,7 @@ def quantize_q4(M, group: int = 128, out=None, stream=None) -> Q4Model:
     elif (out.shape, out.dtype, out.group, out.device) != (tuple(M.shape), M.dtype, group, device):
         raise ValueError("out was made for another shape, dtype, group or device")
     _run("glmm_quantize_q4", sfx, device,
-         (M.data_ptr(), out.codes.data_ptr(), out.scales.data_ptr(), nf, nt, ntasks, out.group))
+         (M.data_ptr(), out._codes_ptr, out._scales_ptr, nf, nt, ntasks, out.group))
     return out
 
 
@@ -440,7 +453,7 @@ def dequantize_q4(model: Q4Model, out=None, stream=None):
     else:
         _need_on(out, "out", model.shape, model.dtype, device)
     _run("glmm_dequantize_q4", SUFFIX[model.dtype], device,
-         (model.codes.data_ptr(), model.scales.data_ptr(), out.data_ptr(), nf, nt, ntasks, model.group))
+         (model._codes_ptr, model._scales_ptr, out.data_ptr(), nf, nt, ntasks, model.group))
     return out
 
 
@@ -470,6 +483,6 @@ def predict_q4(X, model: Q4Model, out=None, workspace=None, stream=None):
         _need_on(out, "out", (nobs, ntasks, nt), dtype, device)
     ws_ptr, ws_bytes = _workspace(workspace, device)
     _run("glmm_predict_q4", SUFFIX[dtype], device,
-         (X.data_ptr(), model.codes.data_ptr(), model.scales.data_ptr(), out.data_ptr(), nf, nt, ntasks, nobs,
+         (X.data_ptr(), model._codes_ptr, model._scales_ptr, out.data_ptr(), nf, nt, ntasks, nobs,
           model.group, ws_ptr, ws_bytes))
     return out
