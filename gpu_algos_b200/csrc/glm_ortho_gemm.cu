@@ -206,7 +206,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     extern __shared__ __align__(1024) unsigned char smem_raw[];
     GemmSmem& sm = *reinterpret_cast<GemmSmem*>(
         reinterpret_cast<unsigned char*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023)));
-    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+    const int tid = threadIdx.x, warp = uniform_warp(), lane = tid & 31;
     const uint32_t rank = cluster_rank();
     const uint32_t half = PAIR ? (rank & 1) : 0;          // which CTA of the pair
     const uint32_t part = PAIR ? (rank >> 1) : rank;      // which share of K
@@ -272,7 +272,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     __syncthreads();
     if (csize > 1) cluster_sync_relaxed();  // the peers' barriers exist before anyone arrives on them
     tc_fence_after();
-    const uint32_t tmem = sm.tmem_base;
+    const uint32_t tmem = __shfl_sync(0xffffffffu, sm.tmem_base, 0);
     volatile int* failed = &sm.failed;
     float* tile = reinterpret_cast<float*>(sm.stage[0]);
     bool finish = true;  // this CTA has (its rows of) the whole sum
@@ -302,7 +302,7 @@ __global__ void __launch_bounds__(kThreads, 1)
             // the copies still in flight land before shared memory is used for anything else
             for (int kb = issued > kStages ? issued - kStages : 0; kb < issued; ++kb)
                 mbar_wait(&sm.full[kb % kStages], uint32_t((kb / kStages) & 1), nullptr);
-        } else if (warp == 1 && lane == 0) {
+        } else if (warp == 1) {
             if (rank == lead) {
                 constexpr uint32_t idesc = instr_desc_f16(kBT, kBN, !kSym);
                 const uint16_t mask = uint16_t(PAIR ? 3u << lead : 0u);
@@ -310,11 +310,12 @@ __global__ void __launch_bounds__(kThreads, 1)
                 const uint32_t right0 = desc_address(saddr(sm.stage[0]) + 2 * kPlaneBytes, kSym ? 16 : kPlaneBytes);
                 for (int kb = 0; kb < nkb; ++kb) {
                     const int s = kb % kStages, buf = kb & 1;
-                    if (kb >= 2 && !mbar_wait_one(&sm.acce[buf], uint32_t(((kb >> 1) - 1) & 1), failed)) break;
-                    if (!mbar_wait_one(&sm.full[s], uint32_t((kb / kStages) & 1), failed)) break;
-                    if (PAIR && !mbar_wait_one(&sm.ready[s], uint32_t((kb / kStages) & 1), failed)) break;
+                    if (kb >= 2 && !mbar_wait_warp(&sm.acce[buf], uint32_t(((kb >> 1) - 1) & 1), failed)) break;
+                    if (!mbar_wait_warp(&sm.full[s], uint32_t((kb / kStages) & 1), failed)) break;
+                    if (PAIR && !mbar_wait_warp(&sm.ready[s], uint32_t((kb / kStages) & 1), failed)) break;
                     tc_fence_after();
                     const uint32_t d = tmem + uint32_t(buf * kBN);
+                    const bool elected = elect_one();
                     // K-major: 16 binary16 = 32 bytes on along the row; 8-row groups 1024 bytes apart.
                     // MN-major: 16 K-rows of 128 bytes on; 8-row groups 1024 bytes, 64-column atoms (hi and lo of
                     // one, then of the next) a plane apart.
@@ -323,29 +324,33 @@ __global__ void __launch_bounds__(kThreads, 1)
                     const uint32_t rh = right0 + uint32_t(s) * (kStageBytes >> 4),
                                    rl = rh + ((kSym ? kPlaneBytes : kPlaneBytes / 2) >> 4);
                     constexpr uint32_t kRight = (kSym ? 32 : 2048) >> 4;
+                    if (elected) {
 #pragma unroll
-                    for (int k = 0; k < kBK / 16; ++k) {
-                        const uint64_t r = desc_join(rh + k * kRight, kRest);
-                        mma_f16<PAIR>(d, desc_join(ll + 2 * k, kRest), r, idesc, k > 0 ? 1u : 0u);
-                        mma_f16<PAIR>(d, desc_join(lh + 2 * k, kRest), desc_join(rl + k * kRight, kRest), idesc, 1u);
+                        for (int k = 0; k < kBK / 16; ++k) {
+                            const uint64_t r = desc_join(rh + k * kRight, kRest);
+                            mma_f16<PAIR>(d, desc_join(ll + 2 * k, kRest), r, idesc, k > 0 ? 1u : 0u);
+                            mma_f16<PAIR>(d, desc_join(lh + 2 * k, kRest), desc_join(rl + k * kRight, kRest), idesc, 1u);
+                        }
+#pragma unroll
+                        for (int k = 0; k < kBK / 16; ++k)
+                            mma_f16<PAIR>(d, desc_join(lh + 2 * k, kRest), desc_join(rh + k * kRight, kRest), idesc, 1u);
+                        commit<PAIR>(&sm.empty[s], mask);
+                        commit<PAIR>(&sm.accf[buf], mask);
                     }
-#pragma unroll
-                    for (int k = 0; k < kBK / 16; ++k)
-                        mma_f16<PAIR>(d, desc_join(lh + 2 * k, kRest), desc_join(rh + k * kRight, kRest), idesc, 1u);
-                    commit<PAIR>(&sm.empty[s], mask);
-                    commit<PAIR>(&sm.accf[buf], mask);
+                    __syncwarp();
                 }
-                commit<PAIR>(&sm.done, mask);
+                if (elect_one()) commit<PAIR>(&sm.done, mask);
+                __syncwarp();
                 // no CTA leaves while a draining warp's arrival is on its way to it
                 for (int b = 0; b < 2 && b < nkb; ++b)
-                    mbar_wait_one(&sm.acce[b], uint32_t(((nkb - b + 1) / 2 - 1) & 1), failed);
+                    mbar_wait_warp(&sm.acce[b], uint32_t(((nkb - b + 1) / 2 - 1) & 1), failed);
             }
-            mbar_wait_one(&sm.done, 0, nullptr);
+            mbar_wait_warp(&sm.done, 0, nullptr);
         } else if (PAIR && warp == 2 && lane == 0 && rank != lead) {
             // tells the even CTA that this CTA's copies of a stage have landed
             for (int kb = 0; kb < nkb; ++kb) {
                 const int s = kb % kStages;
-                if (!mbar_wait_one(&sm.full[s], uint32_t((kb / kStages) & 1), failed)) break;
+                if (!mbar_wait(&sm.full[s], uint32_t((kb / kStages) & 1), failed)) break;
                 fence_proxy_async();
                 mbar_arrive_rank(&sm.ready[s], lead);
             }

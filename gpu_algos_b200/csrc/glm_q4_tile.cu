@@ -122,7 +122,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     extern __shared__ __align__(1024) unsigned char smem_raw[];
     TileSmem<T, N>& sm = *reinterpret_cast<TileSmem<T, N>*>(
         reinterpret_cast<unsigned char*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023)));
-    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+    const int tid = threadIdx.x, warp = uniform_warp(), lane = tid & 31;
     const uint32_t rank = cluster_rank(), half = rank & 1, part = rank >> 1, lead = rank & ~1u;
     const int csize = 2 * a.splits;
     const int64_t unit = blockIdx.x / unsigned(csize);
@@ -163,7 +163,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     __syncthreads();
     cluster_sync_relaxed();  // the peers' barriers exist before anyone arrives on them
     tc_fence_after();
-    const uint32_t tmem = sm.tmem_base;
+    const uint32_t tmem = __shfl_sync(0xffffffffu, sm.tmem_base, 0);
     volatile int* failed = &sm.failed;
     float* part_sums = reinterpret_cast<float*>(sm.stage[0]);  // [observation][target]
 
@@ -185,7 +185,7 @@ __global__ void __launch_bounds__(kThreads, 1)
             // the copies still in flight land before shared memory is used for anything else
             for (int st = issued > kStages ? issued - kStages : 0; st < issued; ++st)
                 mbar_wait(&sm.xfull[st % kStages], uint32_t((st / kStages) & 1), nullptr);
-        } else if (warp == 1 && lane == 0) {
+        } else if (warp == 1) {
             if (rank == lead) {
                 constexpr uint32_t idesc = instr_desc_16<H>(256, N);
                 const uint16_t mask = uint16_t(3u << lead);
@@ -193,13 +193,13 @@ __global__ void __launch_bounds__(kThreads, 1)
                 bool ok = true;
                 for (int st = 0; st < nst && ok; ++st) {
                     const int s = st % kStages;
-                    if (!(ok = mbar_wait_one(&sm.ready[s], uint32_t((st / kStages) & 1), failed))) break;
+                    if (!(ok = mbar_wait_warp(&sm.ready[s], uint32_t((st / kStages) & 1), failed))) break;
 #pragma unroll
                     for (int j = 0; j < kSub; ++j) {
                         const int kb = st * kSub + j, grp = kb >> a.group_shift, buf = grp & 1;
                         const bool first = (kb & (gb - 1)) == 0;
                         if (first && grp >= 2 &&
-                            !(ok = mbar_wait_one(&sm.acce[buf], uint32_t(((grp >> 1) - 1) & 1), failed)))
+                            !(ok = mbar_wait_warp(&sm.acce[buf], uint32_t(((grp >> 1) - 1) & 1), failed)))
                             break;
                         tc_fence_after();
                         // K-major: 16 features = 32 bytes on along the row; 8-row groups 1024 bytes apart
@@ -208,29 +208,33 @@ __global__ void __launch_bounds__(kThreads, 1)
                         const uint32_t x = stage0 + uint32_t(s) * (S::kStageBytes >> 4) +
                                            ((kSub * kATileBytes + j * S::kXBytes) >> 4);
                         const uint32_t d = tmem + uint32_t(buf * N);
+                        if (elect_one()) {
 #pragma unroll
-                        for (int q = S::kTerms - 1; q >= 0; --q)
+                            for (int q = S::kTerms - 1; q >= 0; --q)
 #pragma unroll
-                            for (int k = 0; k < kBK / 16; ++k)
-                                mma_pair(d, desc_join(w + 2 * k, kRest),
-                                         desc_join(x + q * (S::kXTermBytes >> 4) + 2 * k, kRest), idesc,
-                                         q == S::kTerms - 1 && k == 0 ? uint32_t(!first) : 1u);
-                        if ((kb & (gb - 1)) == gb - 1) commit_pair(&sm.accf[buf], mask);
+                                for (int k = 0; k < kBK / 16; ++k)
+                                    mma_pair(d, desc_join(w + 2 * k, kRest),
+                                             desc_join(x + q * (S::kXTermBytes >> 4) + 2 * k, kRest), idesc,
+                                             q == S::kTerms - 1 && k == 0 ? uint32_t(!first) : 1u);
+                            if ((kb & (gb - 1)) == gb - 1) commit_pair(&sm.accf[buf], mask);
+                            if (j == kSub - 1) commit_pair(&sm.empty[s], mask);
+                        }
+                        __syncwarp();
                     }
-                    commit_pair(&sm.empty[s], mask);
                 }
-                commit_pair(&sm.done, mask);
+                if (elect_one()) commit_pair(&sm.done, mask);
+                __syncwarp();
                 // no CTA leaves while a draining warp's arrival is on its way to it
                 const int ngrp = nkb >> a.group_shift;
                 for (int b = 0; b < 2 && b < ngrp; ++b)
-                    mbar_wait_one(&sm.acce[b], uint32_t(((ngrp - b + 1) / 2 - 1) & 1), failed);
+                    mbar_wait_warp(&sm.acce[b], uint32_t(((ngrp - b + 1) / 2 - 1) & 1), failed);
             }
-            mbar_wait_one(&sm.done, 0, nullptr);
+            mbar_wait_warp(&sm.done, 0, nullptr);
         } else if (warp == 2 && lane == 0) {
             // tells the even CTA that this CTA's copies of a stage have landed
             for (int st = 0; st < nst; ++st) {
                 const int s = st % kStages;
-                if (!mbar_wait_one(&sm.xfull[s], uint32_t((st / kStages) & 1), failed)) break;
+                if (!mbar_wait(&sm.xfull[s], uint32_t((st / kStages) & 1), failed)) break;
                 fence_proxy_async();
                 mbar_arrive_rank(&sm.ready[s], lead);
             }

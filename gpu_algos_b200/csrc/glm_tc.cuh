@@ -66,17 +66,24 @@ __device__ __forceinline__ bool mbar_wait(unsigned long long* b, uint32_t parity
     return true;
 }
 
-// The same for a role that one thread plays, on whose path every instruction lies: the clock is read only when
-// the barrier is not there yet.
-__device__ __forceinline__ bool mbar_wait_one(unsigned long long* b, uint32_t parity, volatile int* failed) {
-    return mbar_test(b, parity) || mbar_wait(b, parity, failed);
-}
-
 // The same for a whole warp, which comes out of it converged (what follows -- TMEM loads, an arrival for the
 // warp -- needs that) and of one mind.
 __device__ __forceinline__ bool mbar_wait_warp(unsigned long long* b, uint32_t parity, volatile int* failed) {
+    if (__all_sync(0xffffffffu, mbar_test(b, parity))) return true;
     const bool ok = mbar_wait(b, parity, failed);
     return __all_sync(0xffffffffu, ok) != 0;
+}
+
+// The warp of this thread as a value that the compiler knows to be the same in all its lanes.  A role that
+// branches on it and loops as a whole warp keeps its descriptors in uniform registers, which the MMA reads; with
+// one lane of a divergent branch every operand of every MMA went through a move first, and issuing one took 100
+// to 170 clocks.
+__device__ __forceinline__ int uniform_warp() { return __shfl_sync(0xffffffffu, int(threadIdx.x) >> 5, 0); }
+// One lane of a converged warp.
+__device__ __forceinline__ bool elect_one() {
+    uint32_t p;
+    asm volatile("{\n\t.reg .pred p;\n\telect.sync _|p, 0xffffffff;\n\tselp.u32 %0, 1, 0, p;\n\t}" : "=r"(p));
+    return p != 0;
 }
 
 __device__ __forceinline__ void fence_proxy_async() { asm volatile("fence.proxy.async.shared::cta;" ::: "memory"); }
