@@ -52,8 +52,7 @@ struct GemmSmem {
     alignas(1024) unsigned char stage[kStages][kStageBytes];  // later the float tile
     unsigned long long full[kStages];
     unsigned long long ready[kStages];  // (even CTA of a pair) the odd CTA's copies have landed
-    unsigned long long empty[kStages];
-    unsigned long long accf[2];
+    unsigned long long empty[kStages];  // the stage's MMAs have retired: free for the next copies, sums to be drained
     unsigned long long acce[2];
     unsigned long long done;
     uint32_t tmem_base;
@@ -246,10 +245,7 @@ __global__ void __launch_bounds__(kThreads, 1)
             mbar_init(&sm.ready[s], 1);
             mbar_init(&sm.empty[s], 1);
         }
-        for (int b = 0; b < 2; ++b) {
-            mbar_init(&sm.accf[b], 1);
-            mbar_init(&sm.acce[b], (PAIR ? 2 : 1) * kDrainWarps);
-        }
+        for (int b = 0; b < 2; ++b) mbar_init(&sm.acce[b], (PAIR ? 2 : 1) * kDrainWarps);
         mbar_init(&sm.done, 1);
         sm.failed = 0;
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
@@ -335,7 +331,6 @@ __global__ void __launch_bounds__(kThreads, 1)
                         for (int k = 0; k < kBK / 16; ++k)
                             mma_f16<PAIR>(d, desc_join(lh + 2 * k, kRest), desc_join(rh + k * kRight, kRest), idesc, 1u);
                         commit<PAIR>(&sm.empty[s], mask);
-                        commit<PAIR>(&sm.accf[buf], mask);
                     }
                     __syncwarp();
                 }
@@ -364,8 +359,9 @@ __global__ void __launch_bounds__(kThreads, 1)
         for (int i = 0; i < kCols; ++i) sum[i] = 0.0f;
         bool ok = true;
         for (int kb = 0; kb < nkb; ++kb) {
+            // (the stage cannot come round again unseen: its next MMAs wait for this block's drain)
             const int buf = kb & 1;
-            if (!(ok = mbar_wait_warp(&sm.accf[buf], uint32_t((kb >> 1) & 1), failed))) break;
+            if (!(ok = mbar_wait_warp(&sm.empty[kb % kStages], uint32_t((kb / kStages) & 1), failed))) break;
             tc_fence_after();
 #pragma unroll
             for (int h = 0; h < kCols / 32; ++h) {

@@ -57,8 +57,8 @@ struct TileSmem {
     alignas(1024) unsigned char stage[S::kStages][S::kStageBytes];  // later the partial sums
     unsigned long long xfull[S::kStages];  // this CTA's X has landed
     unsigned long long ready[S::kStages];  // (even CTA) X and operands of both CTAs are there
-    unsigned long long empty[S::kStages];
-    unsigned long long accf[2];
+    unsigned long long empty[S::kStages];  // the stage's MMAs have retired
+    unsigned long long accf;               // the first block's, where a stage holds two groups of features
     unsigned long long acce[2];
     unsigned long long done;
     uint32_t tmem_base;
@@ -144,10 +144,8 @@ __global__ void __launch_bounds__(kThreads, 1)
             mbar_init(&sm.ready[s], 2 * (kMakeWarps + 1));
             mbar_init(&sm.empty[s], 1);
         }
-        for (int b = 0; b < 2; ++b) {
-            mbar_init(&sm.accf[b], 1);
-            mbar_init(&sm.acce[b], 2 * kDrainWarps);
-        }
+        for (int b = 0; b < 2; ++b) mbar_init(&sm.acce[b], 2 * kDrainWarps);
+        mbar_init(&sm.accf, 1);
         mbar_init(&sm.done, 1);
         sm.failed = 0;
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
@@ -216,8 +214,8 @@ __global__ void __launch_bounds__(kThreads, 1)
                                     mma_pair(d, desc_join(w + 2 * k, kRest),
                                              desc_join(x + q * (S::kXTermBytes >> 4) + 2 * k, kRest), idesc,
                                              q == S::kTerms - 1 && k == 0 ? uint32_t(!first) : 1u);
-                            if ((kb & (gb - 1)) == gb - 1) commit_pair(&sm.accf[buf], mask);
                             if (j == kSub - 1) commit_pair(&sm.empty[s], mask);
+                            else if (gb == 1) commit_pair(&sm.accf, mask);
                         }
                         __syncwarp();
                     }
@@ -259,7 +257,13 @@ __global__ void __launch_bounds__(kThreads, 1)
             const float s = to_arith<float>(next);
             sc += kQ4Rows;
             if (live && grp + 1 < ngrp) next = *sc;
-            if (!(ok = mbar_wait_warp(&sm.accf[buf], uint32_t((grp >> 1) & 1), failed))) break;
+            // A group is complete with its last block's stage (which cannot come round again unseen: its next MMAs
+            // wait for this group's drain) or, where two groups share a stage, with the first block.
+            const int last = ((grp + 1) << a.group_shift) - 1, st = last / kSub;
+            const bool whole = last % kSub == kSub - 1;
+            if (!(ok = mbar_wait_warp(whole ? &sm.empty[st % kStages] : &sm.accf,
+                                      uint32_t((whole ? st / kStages : grp >> 1) & 1), failed)))
+                break;
             tc_fence_after();
             // the next sixteen columns load while these are added
             uint32_t r[2][16];
