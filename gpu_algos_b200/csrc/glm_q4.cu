@@ -100,7 +100,7 @@ __device__ __forceinline__ uint32_t nearest_code(float w, float s, float inv, fl
 // One warp per (task, 16 targets, group).  A group's largest magnitude is a maximum over the four lanes of
 // a target.  One pass: the weights in, codes and scales out.
 template <typename T, int GROUP>
-__global__ void __launch_bounds__(kThreads)
+__global__ void __launch_bounds__(kThreads, 2)
     q4_quantize_kernel(const T* __restrict__ M, uint4* __restrict__ codes, T* __restrict__ scales, int64_t nf,
                        int64_t nt, int64_t nrb, int64_t ncb, int64_t ngroups, int64_t total, bool vec) {
     constexpr int kBlocks = GROUP / kQ4Cols;
@@ -588,12 +588,15 @@ int q4_dequantize(const void* codes, const T* scales, T* M, int64_t nf, int64_t 
     return launch_status();
 }
 
-// Up to this many observations go through the stream kernel.
-constexpr int64_t kStreamMost = 16;
+// Up to this many observations go through the stream kernel.  At 16384 x 4096 both sides took, stream and tile:
+// bfloat16 17.4 and 20.9 us at 9 observations, 21.9 and 20.9 at 16; float, whose three terms take three times the
+// products, 32 and 26.3 us at 9.
+template <typename T>
+constexpr int64_t kStreamMost = sizeof(T) == 2 ? 16 : 8;
 
 template <typename T>
 size_t q4_predict_workspace(int64_t nf, int64_t nt, int64_t ntasks, int64_t nobs, int group) {
-    return nobs <= kStreamMost ? 0 : q4_tile_workspace<T>(nf, ntasks, nobs);
+    return nobs <= kStreamMost<T> ? 0 : q4_tile_workspace<T>(nf, ntasks, nobs);
 }
 
 template <typename T>
@@ -601,7 +604,7 @@ int q4_predict(const T* X, const void* codes, const T* scales, T* Yhat, int64_t 
                int64_t nobs, int group, void* ws, size_t ws_bytes, cudaStream_t stream) {
     const int64_t nrb = q4_row_blocks(nt), ncb = q4_col_blocks(nf), ng = q4_groups(nf, group);
     if (nrb > (1 << 27) || ncb > (1 << 20)) return GLMB_ERR_TOO_LARGE;
-    if (nobs > kStreamMost) {
+    if (nobs > kStreamMost<T>) {
         set_last_path("q4_tile");
         return q4_tile_predict<T>(X, codes, scales, Yhat, nf, nt, ntasks, nobs, group, whole_pieces(X, nf, 16), ws,
                                   ws_bytes, stream);
@@ -609,8 +612,9 @@ int q4_predict(const T* X, const void* codes, const T* scales, T* Yhat, int64_t 
     StreamArgs a{nf, nt, ntasks, nobs, 0, int(nrb), int(ncb), int(ng), 0, 0, 0, group == 64 ? 0 : 1, 0,
                  whole_pieces(X, nf, 16)};
     set_last_path("q4_stream");
-    if (nobs <= 8) return stream_predict<T, 1>(X, codes, scales, Yhat, a, stream);
-    return stream_predict<T, 2>(X, codes, scales, Yhat, a, stream);
+    if constexpr (kStreamMost<T> > 8)
+        if (nobs > 8) return stream_predict<T, 2>(X, codes, scales, Yhat, a, stream);
+    return stream_predict<T, 1>(X, codes, scales, Yhat, a, stream);
 }
 
 #define GLMB_INSTANTIATE_Q4(T)                                                                                \
