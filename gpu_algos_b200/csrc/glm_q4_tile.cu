@@ -285,12 +285,17 @@ __global__ void __launch_bounds__(kThreads, 1)
         if (a.splits == 1) {
             // neighbouring lanes on neighbouring targets
             if (target < a.nt) {
+                const int64_t first = n0 + side * kCols, step = a.ntasks * a.nt;
+                const int left = int(min(int64_t(kCols), a.nobs - first));
+                T* to = Yhat + (first * a.ntasks + task) * a.nt + target;
+                if (ok) {
 #pragma unroll
-                for (int i = 0; i < kCols; ++i) {
-                    const int64_t obs = n0 + side * kCols + i;
-                    if (obs < a.nobs)
-                        Yhat[(obs * a.ntasks + task) * a.nt + target] =
-                            from_arith<T>(ok ? sum[i] : __int_as_float(0x7fc00000));
+                    for (int i = 0; i < kCols; ++i) {
+                        if (i < left) *to = from_arith<T>(sum[i]);
+                        to += step;
+                    }
+                } else {
+                    for (int i = 0; i < left; ++i, to += step) *to = from_arith<T>(__int_as_float(0x7fc00000));
                 }
             }
         } else if (ok) {
