@@ -1,5 +1,6 @@
 """B200-native (sm_100a) GLM path of gpu_algos: predict, gradient and the
-elastic-net proximal-gradient fit, behind a C ABI (include/glm_b200.h).
+elastic-net proximal-gradient fit, behind a C ABI (include/glm_b200.h), with
+orthogonalised updates and 4-bit models beside them (include/glm_matrix_b200.h).
 
 Submodules
 ----------

@@ -14,6 +14,12 @@
 // slice of columns in shared memory, forms its share of the first product,
 // sums the shares of all in rank order over distributed shared memory, runs
 // the m x m chain (every CTA its own copy) and multiplies its slice by P.
+//
+// 64 tasks of 16 x 256 in float: about 6 us on the GPU (8.5 us a call from
+// Python), 162 us as three product kernels a step; bound by the chain's 14
+// dependent products of a few hundred clocks and the cluster's two meetings.
+// m <= 32: beyond, the chain (17 products of m^3 in double on one SM) would take
+// longer than the tensor cores' launches.
 #include <algorithm>
 
 #include "glm_ortho.cuh"

@@ -98,7 +98,9 @@ __device__ __forceinline__ uint32_t nearest_code(float w, float s, float inv, fl
 }
 
 // One warp per (task, 16 targets, group).  A group's largest magnitude is a maximum over the four lanes of
-// a target.  One pass: the weights in, codes and scales out.
+// a target.  One pass: the weights in, codes and scales out.  16384 x 4096 bfloat16 in groups of 128: 57 us, 2.9
+// TB/s of the 6.5 that a copy reaches; bound by latency (two CTAs to an SM, for the 64 weights of a lane).  Held
+// as 16-bit values with three CTAs to an SM, or with the next group's loads ahead, it took 64 and 85 us.
 template <typename T, int GROUP>
 __global__ void __launch_bounds__(kThreads, 2)
     q4_quantize_kernel(const T* __restrict__ M, uint4* __restrict__ codes, T* __restrict__ scales, int64_t nf,
@@ -193,7 +195,7 @@ __device__ __forceinline__ void store_piece(T* dst, const uint32_t* w) {
     else *reinterpret_cast<uint2*>(dst) = make_uint2(w[0], w[1]);
 }
 
-// One warp per block of codes: M = q*s, rounded to T.
+// One warp per block of codes: M = q*s, rounded to T.  16384 x 4096 bfloat16: 31 us, 5.5 TB/s.
 template <typename T>
 __global__ void __launch_bounds__(kThreads)
     q4_dequantize_kernel(const uint4* __restrict__ codes, const T* __restrict__ scales, T* __restrict__ M, int64_t nf,
@@ -265,6 +267,13 @@ __global__ void __launch_bounds__(kThreads)
 // a row block go to a slot of its own, and a row block's slots are added up
 // in the order of the warps.  Models with fewer row blocks than SMs share the
 // features out over the CTAs of a cluster as well.
+//
+// 16384 x 4096 in groups of 128, bfloat16: 12.1 us for one observation (5.3 us
+// of codes and scales at HBM's copy rate), 16.2 for 8, 21.9 for 16.  About 110
+// instructions per 128 features of a row block, the half of them the codes'
+// unpacking, share the time with the start and the sums at the end (3 to 4 us).
+// A warp to a row block, its features shared over a cluster of four CTAs, took
+// 18 us: two waves of CTAs, and its index arithmetic as long as its work.
 
 constexpr int kStreamWarps = 16, kStreamThreads = kStreamWarps * 32;
 constexpr int kStreamAhead = 4;   // pairs of blocks (128 features) in flight per warp

@@ -11,12 +11,19 @@
 // of the eight draining warps), to float registers: the scale multiplies a sum
 // of whole-number products and no weight is ever rounded.
 // float observations are three bfloat16 terms with products of their own.
-//
-// Bound by the tensor core at large N (512 clocks of MMA per 64 features at
-// N = 256, against about 450 for making the codes into operands and 40 bytes
-// a clock from L2), by the making of operands at small N.
-// Few tiles share the features out over the pairs of a cluster; their partial
+// Few tiles share the features out over two pairs of a cluster; their partial
 // sums meet in distributed shared memory in rank order.
+//
+// What bounds it.  128 features at N = 256 are eight MMAs of 128 clocks; they
+// take about 1350: making the operands (two blocks of codes by each warp, 800 to
+// 1000 clocks), draining (640) and issuing the MMAs all run beside each other.
+// At small N an MMA still takes its 256 rows about 85 clocks.  16384 targets x
+// 4096 features, bfloat16: 20.4 us at 17 observations, 24 at 128, 237 at 2048
+// (1.16 PFLOP/s, 0.84 of cuBLAS sustained).  Measured and not kept: the operand
+// in tensor memory instead of shared memory (it leaves room for N = 192 at
+// most: 408 us against 311 then), two sets of making warps (no gain: the MMA
+// warp is the longest path at small N), four pairs to a cluster (clusters of
+// eight CTAs do not all fit the GPU at once: 25 us against 18 at 16 x 4096 x 4096).
 #include <algorithm>
 
 #include "glm_q4_device.cuh"
@@ -33,7 +40,7 @@ constexpr int kDrainWarp0 = 4, kDrainWarps = 8;
 constexpr int kMakeWarp0 = kDrainWarp0 + kDrainWarps, kMakeWarps = 8;  // a row block of the tile each
 constexpr int kThreads = (kMakeWarp0 + kMakeWarps) * 32;
 constexpr int kMakeAhead = 4;  // blocks of codes in flight per warp (whole stages)
-constexpr int kMaxSplits = 2;  // pairs of a cluster; clusters of eight CTAs did not all fit the GPU at once
+constexpr int kMaxSplits = 2;  // pairs of a cluster
 // 640 threads launch with 96 registers each; control and making warps give to those that drain
 constexpr uint32_t kRegsControl = 40, kRegsDrain = 168, kRegsMake = 48;
 static_assert(128 * kRegsControl + 256 * kRegsDrain + 256 * kRegsMake <= kThreads * 96, "register split");
@@ -483,8 +490,8 @@ int q4_tile_predict(const T* X, const void* codes, const T* scales, T* Yhat, int
     TileArgs a{nt, ntasks, nobs, q4_row_blocks(nt), int(q4_col_blocks(nf)), int(q4_groups(nf, group)), 0, 0, 1,
                group == 64 ? 0 : 1};
     a.tiles_m = int((nt + 255) / 256);
-    // The cut with the least estimated time, in clocks: a block of features takes 2 N clocks of MMA a term, and
-    // no less than the 450 of making its operands; a tile 5000 besides, and its outputs.
+    // The cut with the least estimated time, in clocks: a block of features takes 2 N clocks of MMA a term and no
+    // less than the 450 of making its operands; a tile 5000 besides, and its outputs.
     int best_n = 0;
     double least = 0.0;
     for (int n = 32; n <= 256; n *= 2) {
