@@ -84,6 +84,16 @@ int step_impl(T* M, const T* grad, float* V, int64_t nf, int64_t nt, int64_t nta
     return ortho_run<T>(grad, V, M, nf, nt, ntasks, plan, &up, ws, ws_bytes, stream);
 }
 
+// Whether an array lies apart from a 4-bit model's codes and scales (and those from one another).
+template <typename T>
+bool apart(const void* p, size_t bytes, const void* codes, const T* scales, int64_t nf, int64_t nt, int64_t ntasks,
+           int group) {
+    const size_t blocks = size_t(ntasks) * size_t(q4_row_blocks(nt));
+    const size_t cb = blocks * size_t(q4_col_blocks(nf)) * kQ4BlockBytes,
+                 sb = blocks * kQ4Rows * size_t(q4_groups(nf, group)) * sizeof(T);
+    return !overlap(p, bytes, codes, cb) && !overlap(p, bytes, scales, sb) && !overlap(codes, cb, scales, sb);
+}
+
 template <typename T>
 int quantize_impl(const T* M, void* codes, T* scales, int64_t nf, int64_t nt, int64_t ntasks, int group,
                   cudaStream_t stream) {
@@ -91,6 +101,8 @@ int quantize_impl(const T* M, void* codes, T* scales, int64_t nf, int64_t nt, in
     if (nf == 0 || nt == 0 || ntasks == 0) return GLMB_OK;
     if (M == nullptr || codes == nullptr || scales == nullptr || !aligned(codes, 16)) return GLMB_ERR_INVALID_VALUE;
     if (!sizes_ok(nf, nt, ntasks)) return GLMB_ERR_TOO_LARGE;
+    if (!apart(M, size_t(nf) * size_t(nt) * size_t(ntasks) * sizeof(T), codes, scales, nf, nt, ntasks, group))
+        return GLMB_ERR_INVALID_VALUE;
     if (const int st = device_check(); st != GLMB_OK) return st;
     return q4_quantize<T>(M, codes, scales, nf, nt, ntasks, group, stream);
 }
@@ -102,6 +114,8 @@ int dequantize_impl(const void* codes, const T* scales, T* M, int64_t nf, int64_
     if (nf == 0 || nt == 0 || ntasks == 0) return GLMB_OK;
     if (M == nullptr || codes == nullptr || scales == nullptr || !aligned(codes, 16)) return GLMB_ERR_INVALID_VALUE;
     if (!sizes_ok(nf, nt, ntasks)) return GLMB_ERR_TOO_LARGE;
+    if (!apart(M, size_t(nf) * size_t(nt) * size_t(ntasks) * sizeof(T), codes, scales, nf, nt, ntasks, group))
+        return GLMB_ERR_INVALID_VALUE;
     if (const int st = device_check(); st != GLMB_OK) return st;
     return q4_dequantize<T>(codes, scales, M, nf, nt, ntasks, group, stream);
 }
@@ -117,7 +131,9 @@ int predict_q4_impl(const T* X, const void* codes, const T* scales, T* Yhat, int
     if (!sizes_ok(nf, nt, ntasks) || !sizes_ok(nf, ntasks, nobs) || !sizes_ok(nt, ntasks, nobs))
         return GLMB_ERR_TOO_LARGE;
     const size_t rows = size_t(ntasks) * size_t(nobs) * sizeof(T);
-    if (nf > 0 && overlap(X, rows * size_t(nf), Yhat, rows * size_t(nt))) return GLMB_ERR_INVALID_VALUE;
+    if (nf > 0 && (overlap(X, rows * size_t(nf), Yhat, rows * size_t(nt)) ||
+                   !apart(Yhat, rows * size_t(nt), codes, scales, nf, nt, ntasks, group)))
+        return GLMB_ERR_INVALID_VALUE;
     if (const int st = device_check(); st != GLMB_OK) return st;
     if (nf == 0) {
         set_last_path("memset");

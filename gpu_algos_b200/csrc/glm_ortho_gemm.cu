@@ -745,11 +745,18 @@ struct Cuts {
 };
 }  // namespace
 
+// What any cut of the three products may take, whatever clusters the device holds: the size a caller asked for
+// while another device was current has to do.
 size_t ortho_partial_bytes(int64_t m, int64_t n, int64_t ntasks) {
-    const Cuts cuts(m, n, ntasks);
+    const int64_t kbn = (n + kBK - 1) / kBK, kbm = (m + kBK - 1) / kBK;
     size_t most = 0;
-    for (const Cut& c : {cuts.gram, cuts.poly, cuts.apply})
-        if (c.halves == 2) most = std::max(most, size_t(c.units * ntasks) * 2 * (c.pair ? 2 * 128 * 256 : 128 * 128) * 4);
+    for (const bool pair : {true, false})
+        for (int product = 0; product < 3; ++product) {
+            const int64_t bt = pair ? 256 : 128, tm = (m + bt - 1) / bt, tn = (n + bt - 1) / bt;
+            const int64_t ctas = (product < 2 ? tm * (tm + 1) / 2 : tm * tn) * ntasks * (pair ? 2 : 1);
+            if (ctas <= kMaxHalved && (product == 0 ? kbn : kbm) >= 4)
+                most = std::max(most, size_t(ctas) * 2 * 128 * (pair ? 256 : 128) * sizeof(float));
+        }
     return most;
 }
 size_t ortho_arrived_bytes() { return size_t(kMaxHalved) * sizeof(int); }

@@ -337,6 +337,7 @@ def orthogonalize(G, steps: int = 5, coefficients=None, out=None, workspace=None
     sfx, device = _matrix_suffix(G.dtype), G.device
     ntasks, nt, nf = _model_dims(G, "G")
     _need_on(G, "G", G.shape, G.dtype, device)
+    steps = int(steps)
     coef = _coefficients(coefficients, steps)
     on = _on(device, stream)
     if on is not None:
@@ -370,6 +371,7 @@ def orthogonal_step(M, grad, momentum, lr: float, mu: float = 0.95, nesterov: bo
     _need_on(momentum, "momentum", M.shape, torch.float32, device)
     if scale is None:
         scale = math.sqrt(max(1.0, nt / nf)) if nf > 0 else 1.0
+    steps = int(steps)
     coef = _coefficients(coefficients, steps)
     on = _on(device, stream)
     if on is not None:

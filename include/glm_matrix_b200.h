@@ -38,7 +38,9 @@ extern "C" {
  * O NaN.
  * GLMB_ERR_INVALID_VALUE also when steps is outside 1..GLMM_MAX_STEPS, or
  * when the coefficients are not finite or let a singular value of X grow past
- * 16 (or |a + b s^2 + c s^4| past 1024).
+ * 16 (or |a + b s^2 + c s^4| past 1024).  GLMB_ERR_TOO_LARGE for more than
+ * 65535 tasks whose matrices have over 32 rows and columns, or a side past 2^30
+ * of such a matrix.
  * ---------------------------------------------------------------------- */
 #define GLMM_MAX_STEPS 16
 

@@ -89,6 +89,34 @@ def test_shapes(shape, dtype):
     assert torch.equal(G, before)
 
 
+# tiles of pairs, K over clusters of sixteen and over two halves, and their tall counterparts
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("shape", [(1, 1300, 2600), (1, 2600, 1300), (1, 100, 9000), (1, 9000, 100), (2, 600, 640),
+                                   (40, 130, 140)])
+def test_cuts(shape, dtype):
+    G = _gradient(shape, dtype, 12)
+    _check(glm.orthogonalize(G), G)
+
+
+def test_wrappers_refuse_what_does_not_fit():
+    G = torch.ones(2, 40, 50, device="cuda")
+    before = capi.launch_count()
+    for bad in (G.transpose(1, 2), G[:, ::2], G.cpu(), G[0], G.double()):
+        with pytest.raises(ValueError):
+            glm.orthogonalize(bad)
+    with pytest.raises(ValueError):
+        glm.orthogonalize(G, out=torch.empty(2, 50, 40, device="cuda"))
+    with pytest.raises(ValueError):
+        glm.orthogonal_step(G, G.half(), torch.zeros_like(G), 0.1)
+    with pytest.raises(ValueError):
+        glm.orthogonal_step(G, torch.ones_like(G), torch.zeros_like(G).half(), 0.1)
+    with pytest.raises(capi.GlmbError):
+        glm.orthogonal_step(G, G, torch.zeros_like(G), 0.1)  # the gradient is the model
+    with pytest.raises(capi.GlmbError):
+        glm.orthogonalize(G, steps=0)
+    assert capi.launch_count() == before
+
+
 @pytest.mark.parametrize("shape", [(2, 16, 100), (2, 150, 130), (1, 700, 300)])
 @pytest.mark.parametrize("coefs", [[(1.5, -0.5, 0.0)] * 3, [(2.0, -1.5, 0.5)] * 12, [DEFAULT],
                                    [(3.0, -4.0, 1.75), (2.0, -1.5, 0.5), (1.875, -1.25, 0.375)],

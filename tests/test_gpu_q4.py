@@ -129,6 +129,35 @@ def test_predict_over_models(shape, group, dtype):
         _check_predict(Y, X, M, group)
 
 
+# longer than shared memory holds at once, more row blocks to a CTA than it takes together, features over clusters
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("shape,nobs", [((1, 2500, 9000), 8), ((1, 2400, 20000), 13), ((1, 16, 70000), 3),
+                                        ((1, 40000, 130), 2), ((1, 40000, 130), 16), ((300, 7, 100), 5),
+                                        ((3, 700, 12000), 40), ((1, 20, 30000), 200)])
+def test_predict_long_and_many(shape, nobs, dtype):
+    for group in (64, 128):
+        Y, X, M, _ = _predict(shape, nobs, dtype, group, 6)
+        _check_predict(Y, X, M, group)
+
+
+def test_wrappers_refuse_what_does_not_fit():
+    q = glm.quantize_q4(torch.ones(2, 3, 8, device="cuda"), 64)
+    before = capi.launch_count()
+    X = torch.ones(4, 2, 8, device="cuda")
+    for bad in (X.half(), X[:, :1], X[:, :, :4], X.transpose(0, 1).contiguous().transpose(0, 1), X.cpu()):
+        with pytest.raises(ValueError):
+            glm.predict_q4(bad, q)
+    with pytest.raises(ValueError):
+        glm.predict_q4(X, q, out=torch.empty(4, 2, 4, device="cuda"))
+    with pytest.raises(ValueError):
+        glm.predict_q4(X, q, workspace=torch.empty(16, dtype=torch.uint8))
+    with pytest.raises(ValueError):
+        glm.quantize_q4(torch.ones(2, 3, 8, device="cuda"), 128, out=q)
+    with pytest.raises(ValueError):
+        glm.dequantize_q4(q, out=torch.empty(2, 3, 8, device="cuda", dtype=torch.float16))
+    assert capi.launch_count() == before
+
+
 def test_predict_without_features_or_observations():
     q = glm.quantize_q4(torch.zeros(2, 3, 0, device="cuda"))
     Y = glm.predict_q4(torch.zeros(4, 2, 0, device="cuda"), q)

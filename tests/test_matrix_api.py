@@ -84,12 +84,17 @@ def test_q4_refusals(sfx):
             assert f(*args, 4, 4, 1, 64, None) == INVALID
         assert f(None, None, None, 0, 4, 1, 64, None) == 0
         assert f(P, Q, R, 1 << 39, 1 << 39, 1, 64, None) == TOO_LARGE
+        for args in ((P, P, R), (P, P + 16, R), (P, Q, P), (P, Q, P + 28), (P, Q, Q + 16)):
+            assert f(*args, 4, 4, 1, 64, None) == INVALID          # overlaps
+    assert quant(Q + 960, Q, R, 4, 4, 1, 64, None) == INVALID  # the weights end inside the codes
+    assert deq(P, Q, P + 992, 4, 4, 1, 64, None) == INVALID
     assert quant(P, Q + 8, R, 4, 4, 1, 64, None) == INVALID   # codes alignment
     assert deq(P + 8, Q, R, 4, 4, 1, 64, None) == INVALID
     Y = 0x90000
     assert pred(P, Q, R, Y, 4, 4, 1, -1, 64, None, 0, None) == INVALID
     assert pred(P, Q, R, Y, 4, 4, 1, 2, 96, None, 0, None) == INVALID
-    for args in ((None, Q, R, Y), (P, None, R, Y), (P, Q, None, Y), (P, Q, R, None), (P, Q, R, P), (P, Q + 4, R, Y)):
+    for args in ((None, Q, R, Y), (P, None, R, Y), (P, Q, None, Y), (P, Q, R, None), (P, Q, R, P), (P, Q + 4, R, Y),
+                 (P, Q, R, Q + 16), (P, Q, R, R), (P, Q, Q + 512, Y)):
         assert pred(*args, 4, 4, 1, 2, 64, None, 0, None) == INVALID
     assert pred(P, Q, R, Y, 4, 4, 1, 2, 64, R + 16, 1 << 20, None) == INVALID
     for nf, nt, ntasks, nobs in ((4, 0, 1, 2), (4, 4, 0, 2), (4, 4, 1, 0)):
