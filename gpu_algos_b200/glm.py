@@ -400,9 +400,15 @@ class Q4Model:
         # one allocation; the scales follow the codes, which are a multiple of 512 bytes
         self._held = torch.empty(codes + count * dtype.itemsize, dtype=torch.uint8, device=device)
         self._codes_bytes = codes
-        self._codes_ptr = self._held.data_ptr()
-        self._scales_ptr = self._codes_ptr + codes
-        self.device = self._held.device
+
+    def _pointers(self):
+        # (asked of the tensor every time: a copied or unpickled model has another one)
+        codes = self._held.data_ptr()
+        return codes, codes + self._codes_bytes
+
+    @property
+    def device(self):
+        return self._held.device
 
     @property
     def codes(self):
@@ -436,7 +442,7 @@ def quantize_q4(M, group: int = 128, out=None, stream=None) -> Q4Model:
     elif (out.shape, out.dtype, out.group, out.device) != (tuple(M.shape), M.dtype, group, device):
         raise ValueError("out was made for another shape, dtype, group or device")
     _run("glmm_quantize_q4", sfx, device,
-         (M.data_ptr(), out._codes_ptr, out._scales_ptr, nf, nt, ntasks, out.group))
+         (M.data_ptr(), *out._pointers(), nf, nt, ntasks, out.group))
     return out
 
 
@@ -455,7 +461,7 @@ def dequantize_q4(model: Q4Model, out=None, stream=None):
     else:
         _need_on(out, "out", model.shape, model.dtype, device)
     _run("glmm_dequantize_q4", SUFFIX[model.dtype], device,
-         (model._codes_ptr, model._scales_ptr, out.data_ptr(), nf, nt, ntasks, model.group))
+         (*model._pointers(), out.data_ptr(), nf, nt, ntasks, model.group))
     return out
 
 
@@ -485,6 +491,6 @@ def predict_q4(X, model: Q4Model, out=None, workspace=None, stream=None):
         _need_on(out, "out", (nobs, ntasks, nt), dtype, device)
     ws_ptr, ws_bytes = _workspace(workspace, device)
     _run("glmm_predict_q4", SUFFIX[dtype], device,
-         (X.data_ptr(), model._codes_ptr, model._scales_ptr, out.data_ptr(), nf, nt, ntasks, nobs,
+         (X.data_ptr(), *model._pointers(), out.data_ptr(), nf, nt, ntasks, nobs,
           model.group, ws_ptr, ws_bytes))
     return out

@@ -140,6 +140,24 @@ def test_predict_long_and_many(shape, nobs, dtype):
         _check_predict(Y, X, M, group)
 
 
+def test_a_copied_model_stands_alone():
+    import copy
+    import io
+
+    M = _model((1, 40, 200), torch.bfloat16)
+    q = glm.quantize_q4(M, 64)
+    X = torch.ones(3, 1, 200, device="cuda", dtype=torch.bfloat16)
+    Y = glm.predict_q4(X, q)
+    twin = copy.deepcopy(q)
+    buf = io.BytesIO()
+    torch.save(q, buf)
+    buf.seek(0)
+    loaded = torch.load(buf, weights_only=False)
+    glm.quantize_q4(torch.zeros_like(M), 64, out=q)  # the first one is overwritten
+    assert torch.equal(glm.predict_q4(X, twin), Y) and torch.equal(glm.predict_q4(X, loaded), Y)
+    assert torch.count_nonzero(glm.predict_q4(X, q)) == 0
+
+
 def test_wrappers_refuse_what_does_not_fit():
     q = glm.quantize_q4(torch.ones(2, 3, 8, device="cuda"), 64)
     before = capi.launch_count()
