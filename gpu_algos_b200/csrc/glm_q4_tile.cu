@@ -406,17 +406,31 @@ __global__ void __launch_bounds__(kThreads, 1)
 template <typename T>
 __global__ void __launch_bounds__(256)
     q4_terms_kernel(const T* __restrict__ X, typename Split16<T>::Type* __restrict__ out, int64_t rows, int64_t nf,
-                    int64_t ld) {
+                    int64_t ld, bool vec) {
     constexpr int kTerms = Split16<T>::kTerms;
     pdl_allow_dependents();
     const int64_t pieces = ld / 8, total = rows * pieces;
     for (int64_t i = int64_t(blockIdx.x) * 256 + threadIdx.x; i < total; i += int64_t(gridDim.x) * 256) {
         const int64_t row = i / pieces, f = (i - row * pieces) * 8;
+        constexpr int kPer = 16 / sizeof(T);
+        T x[8];
+        if (vec) {  // ld == nf rounded up to 8: the last piece may end at nf, on a whole 16 bytes
+#pragma unroll
+            for (int e = 0; e < 8; e += kPer) {
+                T part[kPer] = {};
+                if (f + e < nf) VecLoad<T, kPer>::load(X + row * nf + f + e, part);
+#pragma unroll
+                for (int j = 0; j < kPer; ++j) x[e + j] = part[j];
+            }
+        } else {
+#pragma unroll
+            for (int e = 0; e < 8; ++e) x[e] = f + e < nf ? X[row * nf + f + e] : from_arith<T>(0.0f);
+        }
         alignas(16) typename Split16<T>::Type t[kTerms][8];
 #pragma unroll
         for (int e = 0; e < 8; ++e) {
             typename Split16<T>::Type one[kTerms];
-            split_terms<T>(f + e < nf ? X[row * nf + f + e] : from_arith<T>(0.0f), one);
+            split_terms<T>(x[e], one);
 #pragma unroll
             for (int q = 0; q < kTerms; ++q) t[q][e] = one[q];
         }
@@ -482,7 +496,7 @@ int q4_tile_predict(const T* X, const void* codes, const T* scales, T* Yhat, int
     if (lay_out) {
         H* out = sc.template as<H>();
         const int64_t blocks = std::min<int64_t>(int64_t(sm_count()) * 16, (rows * (ld / 8) + 255) / 256);
-        q4_terms_kernel<T><<<unsigned(std::max<int64_t>(1, blocks)), 256, 0, stream>>>(X, out, rows, nf, ld);
+        q4_terms_kernel<T><<<unsigned(std::max<int64_t>(1, blocks)), 256, 0, stream>>>(X, out, rows, nf, ld, vec);
         count_launch();
         if (const int st = launch_status(); st != GLMB_OK) return st;
         src = out;
