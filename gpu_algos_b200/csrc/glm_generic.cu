@@ -115,10 +115,12 @@ __global__ void __launch_bounds__(kGenTX* kGenTY)
 
 template <typename T, typename P>
 __global__ void __launch_bounds__(256)
-    glm_finalize_kernel(const P* __restrict__ part, int64_t nparts, int64_t total,
+    glm_finalize_kernel(const P* part, int64_t nparts, int64_t total,
                         const T* __restrict__ M, T* __restrict__ grad, double* __restrict__ partial_out,
                         double lambda, double alpha, int reg) {
-    pdl_wait_for_producer();  // the partials are the previous kernel's output
+    // The partials are the previous kernel's output, which may still run when this one starts: `part` is not
+    // __restrict__, as loads of the read-only path are not for memory written while the kernel lives.
+    pdl_wait_for_producer();
     const int lane = threadIdx.x & (kWarp - 1);
     const int64_t nwarps = (int64_t(gridDim.x) * blockDim.x) >> 5;
     for (int64_t e = (int64_t(blockIdx.x) * blockDim.x + threadIdx.x) >> 5; e < total; e += nwarps) {

@@ -99,10 +99,12 @@ __device__ __forceinline__ void put_split2(__half* dst, int64_t plane, float a, 
 
 // X = scale * U / |U| into its planes, for matrices at least as wide as tall: two neighbouring columns to a
 // thread, four rows at a time.  Columns that fill up a row to ld are zero.  Bound by HBM.
+// V and part are not __restrict__: this kernel starts while the one that writes them still runs, so their loads
+// (after the wait) may not take the read-only path.
 template <typename T>
 __global__ void __launch_bounds__(kThreads)
-    ortho_split_kernel(const T* __restrict__ G, const float* __restrict__ V, const double* __restrict__ part, int nparts,
-                       __half* __restrict__ X, int64_t m, int64_t n, int64_t ld, float scale, OrthoUpdate up) {
+    ortho_split_kernel(const T* __restrict__ G, const float* V, const double* part, int nparts, __half* __restrict__ X,
+                       int64_t m, int64_t n, int64_t ld, float scale, OrthoUpdate up) {
     __shared__ double shared;
     pdl_allow_dependents();
     pdl_wait_for_producer();
@@ -129,8 +131,8 @@ __global__ void __launch_bounds__(kThreads)
 // The same of matrices taller than wide, transposed through 64 x 64 tiles.
 template <typename T>
 __global__ void __launch_bounds__(kThreads)
-    ortho_split_tall_kernel(const T* __restrict__ G, const float* __restrict__ V, const double* __restrict__ part,
-                            int nparts, __half* __restrict__ X, int64_t m, int64_t n, int64_t ld, float scale,
+    ortho_split_tall_kernel(const T* __restrict__ G, const float* V, const double* part, int nparts,
+                            __half* __restrict__ X, int64_t m, int64_t n, int64_t ld, float scale,
                             OrthoUpdate up) {
     __shared__ float t[64][65];
     __shared__ double shared;
