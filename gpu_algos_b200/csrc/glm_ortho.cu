@@ -159,9 +159,12 @@ __global__ void __launch_bounds__(kThreads)
     }
 }
 
-// Blocks a task's norm is shared by: enough for the memory system, 4096 elements each at the least.
+// Blocks a task's norm is shared by: enough for the memory system (eight to each of a B200's 148 SMs over all
+// tasks), 4096 elements each at the least.  The number sets the workspace's layout, so it depends on the sizes
+// alone and not on the device that is current when a caller asks.
+constexpr int64_t kNormBlocks = 8 * 148;
 int64_t norm_blocks(int64_t size, int64_t ntasks) {
-    const int64_t most = std::max<int64_t>(1, 8 * int64_t(sm_count()) / std::max<int64_t>(1, ntasks));
+    const int64_t most = std::max<int64_t>(1, kNormBlocks / std::max<int64_t>(1, ntasks));
     return std::max<int64_t>(1, std::min(most, (size + 4095) / 4096));
 }
 
