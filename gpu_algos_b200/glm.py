@@ -331,18 +331,24 @@ def orthogonalize(G, steps: int = 5, coefficients=None, out=None, workspace=None
     ``(ntasks, ntargets, nfeatures)``: X = G/|G|_F (zero stays zero), then
     ``steps`` times X <- aX + (bA + cA^2)X with A = X X^T on the shorter side.
 
-    ``coefficients``: one (a, b, c) or one per step, by default (3.4445,
+    ``coefficients``: one (a, b, c) or one per step (any iterable of them), by default (3.4445,
     -4.7750, 2.0315), which brings the singular values near 1 in five steps.
     ``out`` may be ``G``."""
     sfx, device = _matrix_suffix(G.dtype), G.device
-    ntasks, nt, nf = _model_dims(G, "G")
+    _model_dims(G, "G")
     _need_on(G, "G", G.shape, G.dtype, device)
     steps = int(steps)
     coef = _coefficients(coefficients, steps)
     on = _on(device, stream)
     if on is not None:
         with on:
-            return orthogonalize(G, steps, coefficients, out, workspace)
+            return _orthogonalize(G, sfx, device, steps, coef, out, workspace)
+    return _orthogonalize(G, sfx, device, steps, coef, out, workspace)
+
+
+def _orthogonalize(G, sfx, device, steps, coef, out, workspace):
+    # (on the current stream of `device`; coefficients may be an iterator, so they come as the array made of them)
+    ntasks, nt, nf = G.shape
     if out is None:
         out = torch.empty_like(G)
     else:
@@ -373,15 +379,15 @@ def orthogonal_step(M, grad, momentum, lr: float, mu: float = 0.95, nesterov: bo
         scale = math.sqrt(max(1.0, nt / nf)) if nf > 0 else 1.0
     steps = int(steps)
     coef = _coefficients(coefficients, steps)
+    ws_ptr, ws_bytes = _workspace(workspace, device)
+    args = (M.data_ptr(), grad.data_ptr(), momentum.data_ptr(), nf, nt, ntasks, float(lr), float(mu),
+            float(weight_decay), float(scale), capi.STEP_NESTEROV if nesterov else 0, coef, steps, ws_ptr, ws_bytes)
     on = _on(device, stream)
     if on is not None:
         with on:
-            return orthogonal_step(M, grad, momentum, lr, mu, nesterov, weight_decay, scale, steps, coefficients,
-                                   workspace)
-    ws_ptr, ws_bytes = _workspace(workspace, device)
-    _run("glmm_orthogonal_step", sfx, device,
-         (M.data_ptr(), grad.data_ptr(), momentum.data_ptr(), nf, nt, ntasks, float(lr), float(mu),
-          float(weight_decay), float(scale), capi.STEP_NESTEROV if nesterov else 0, coef, steps, ws_ptr, ws_bytes))
+            _run("glmm_orthogonal_step", sfx, device, args)
+    else:
+        _run("glmm_orthogonal_step", sfx, device, args)
     return M
 
 
