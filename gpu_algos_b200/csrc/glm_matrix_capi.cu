@@ -68,6 +68,10 @@ int step_impl(T* M, const T* grad, float* V, int64_t nf, int64_t nt, int64_t nta
     if (nf < 0 || nt < 0 || ntasks < 0 || (flags & ~GLMM_STEP_NESTEROV) != 0) return GLMB_ERR_INVALID_VALUE;
     if (!std::isfinite(lr) || !std::isfinite(mu) || !std::isfinite(weight_decay) || !std::isfinite(scale))
         return GLMB_ERR_INVALID_VALUE;
+    // what the kernels take, as floats; finite arguments can still have products that are not
+    const OrthoUpdate up{float(mu), (flags & GLMM_STEP_NESTEROV) != 0, float(1.0 - lr * weight_decay),
+                         float(lr * scale)};
+    if (!std::isfinite(up.mu) || !std::isfinite(up.keep) || !std::isfinite(up.rate)) return GLMB_ERR_INVALID_VALUE;
     OrthoSteps plan;
     int st = ortho_plan_steps(coefficients, steps, &plan);
     if (st != GLMB_OK) return st;
@@ -79,8 +83,6 @@ int step_impl(T* M, const T* grad, float* V, int64_t nf, int64_t nt, int64_t nta
         overlap(grad, n * sizeof(T), V, n * sizeof(float)))
         return GLMB_ERR_INVALID_VALUE;
     if ((st = device_check()) != GLMB_OK) return st;
-    const OrthoUpdate up{float(mu), (flags & GLMM_STEP_NESTEROV) != 0, float(1.0 - lr * weight_decay),
-                         float(lr * scale)};
     return ortho_run<T>(grad, V, M, nf, nt, ntasks, plan, &up, ws, ws_bytes, stream);
 }
 

@@ -48,7 +48,9 @@ extern "C" {
  *   V <- mu V + grad          (V: float, the model's shape)
  *   U  = grad + mu V with GLMM_STEP_NESTEROV, V otherwise
  *   M <- (1 - lr*weight_decay) M - lr*scale * O(U)
- * with O the orthogonalisation above.  M, grad and V are distinct arrays. */
+ * with O the orthogonalisation above.  M, grad and V are distinct arrays.
+ * GLMB_ERR_INVALID_VALUE also when mu, 1 - lr*weight_decay or lr*scale is not
+ * finite as a float. */
 #define GLMM_STEP_NESTEROV 0x1u
 
 /* The workspace serves both entry points. */
