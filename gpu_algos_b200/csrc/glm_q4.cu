@@ -455,10 +455,10 @@ __global__ void __launch_bounds__(kStreamThreads, 1)
                     uint32_t frag[2][4][4];
 #pragma unroll
                     for (int h = 0; h < 2; ++h) {
-                        code_pairs<H>(w[j][h].x, frag[h][0]);
-                        code_pairs<H>(w[j][h].y, frag[h][1]);
-                        code_pairs<H>(w[j][h].z, frag[h][2]);
-                        code_pairs<H>(w[j][h].w, frag[h][3]);
+                        code_pairs<H, kCodeDown<H>>(w[j][h].x, frag[h][0]);
+                        code_pairs<H, kCodeDown<H>>(w[j][h].y, frag[h][1]);
+                        code_pairs<H, kCodeDown<H>>(w[j][h].z, frag[h][2]);
+                        code_pairs<H, kCodeDown<H>>(w[j][h].w, frag[h][3]);
                     }
                     fetch(w[j]);
                     float acc[NT][4] = {};
@@ -511,7 +511,7 @@ __global__ void __launch_bounds__(kStreamThreads, 1)
                     const float* from = slots + (k * kSlots + slot) * kSlotFloats + o * kSlotLd + t % kQ4Rows;
                     v += ranks > 1 ? ld_cluster_f32(from, p) : *from;
                 }
-            if (target < a.nt) Yhat[((obs0 + o) * a.ntasks + task) * a.nt + target] = from_arith<T>(v);
+            if (target < a.nt) Yhat[((obs0 + o) * a.ntasks + task) * a.nt + target] = from_arith<T>(v * kCodeUp<H>);
         }
         if (ranks > 1) cluster_sync_relaxed();  // the peers have read this CTA's sums
         else if (rb0 + kStreamRows < rb_end) __syncthreads();

@@ -298,7 +298,7 @@ __global__ void __launch_bounds__(kThreads, 1)
                 if (ok) {
 #pragma unroll
                     for (int i = 0; i < kCols; ++i) {
-                        if (i < left) *to = from_arith<T>(sum[i]);
+                        if (i < left) *to = from_arith<T>(sum[i] * kCodeUp<H>);
                         to += step;
                     }
                 } else {
@@ -353,7 +353,7 @@ __global__ void __launch_bounds__(kThreads, 1)
 #pragma unroll
                         for (int k = 0; k < 4; ++k) {
                             uint32_t p[4];
-                            code_pairs<H>(word[k], p);
+                            code_pairs<H, kCodeDown<H>>(word[k], p);
                             *reinterpret_cast<uint2*>(tile + at[k]) = make_uint2(p[0], p[2]);
                             *reinterpret_cast<uint2*>(tile + at[k] + 8 * 128) = make_uint2(p[1], p[3]);
                         }
@@ -390,7 +390,7 @@ __global__ void __launch_bounds__(kThreads, 1)
 #pragma unroll
                 for (int p = 1; p < kMaxSplits; ++p)
                     if (p < a.splits) v[0] += v[p];
-                Yhat[(obs * a.ntasks + task) * a.nt + target] = from_arith<T>(bad ? __int_as_float(0x7fc00000) : v[0]);
+                Yhat[(obs * a.ntasks + task) * a.nt + target] = from_arith<T>(bad ? __int_as_float(0x7fc00000) : v[0] * kCodeUp<H>);
             }
         }
     }

@@ -99,7 +99,10 @@ int64_t glmm_q4_scales_count(int64_t nfeatures, int64_t ntargets, int64_t ntasks
 
 /* quantize: codes and scales of M.  dequantize: M = q*s, rounded to the type.
  * predict: Yhat[t, task, obs] = sum_f q[f, t, task]*s * X[f, task, obs], sums
- * in float, one rounding to the type. */
+ * in float, one rounding to the type.  A group's sum of q*X is formed before it
+ * is multiplied by s, 2^-10 of it, so that no finite X takes it past float's
+ * range.  Bits of a float X below 2^-133 are lost, and a float or bfloat16
+ * result below 2^-116 is summed in steps of 2^-139. */
 #define GLMM_DECLARE_Q4(SFX, T)                                                         \
     int glmm_quantize_q4_##SFX(const T* M, void* codes, T* scales, int64_t nfeatures,   \
                                int64_t ntargets, int64_t ntasks, int group,             \
