@@ -5,7 +5,8 @@
 // Operands are pairs of binary16 values, hi = the value rounded to nearest and
 // lo = the rest rounded to nearest, after a scaling by a power of two that the
 // host derives from the bound on X's singular values (glm_ortho.cuh): 22
-// significant bits, and an absolute 2^-25 of the scaled unit at the least.  A
+// significant bits where the low value is normal (down to 2^-17 of the bound),
+// an error of 2^-25 of the scaled unit (2^-39 of the bound) below.  A
 // product takes three MMAs (hi*lo + lo*hi + hi*hi; the dropped lo*lo is 2^-22
 // of the product), at twice the rate of tf32 and half its bytes.  Normalised
 // iterates make this possible: nothing in X, A or B can leave binary16's range.

@@ -33,9 +33,13 @@ extern "C" {
  * with (a, b, c) = coefficients[3*k ..] of step k, a host array of 3*steps
  * doubles that is read during the call; NULL stands for (3.4445, -4.7750,
  * 2.0315) in every step, which brings the singular values of X near 1 in five
- * steps.  O may be G.  Iterates carry at least 22 significant bits and sums are
- * float or wider, whatever the type; a NaN or infinity in a task's G makes that task's
- * O NaN.
+ * steps.  O may be G.  Sums are float or wider, whatever the type.  Where both
+ * sides are longer than 32, iterates carry 22 significant bits down to 2^-17 of
+ * the largest singular value that the coefficients let them have (1 at first;
+ * counted as 1e-3 where it is less) and steps of 2^-38 of it below that: the
+ * entries of a feature a million times smaller than the others keep a few bits
+ * of their own.  Shorter matrices are worked on in double.  A NaN or infinity in
+ * a task's G makes that task's O NaN.
  * GLMB_ERR_INVALID_VALUE also when steps is outside 1..GLMM_MAX_STEPS, or
  * when the coefficients are not finite or let a singular value of X grow past
  * 16 (or |a + b s^2 + c s^4| past 1024).  GLMB_ERR_TOO_LARGE for more than
