@@ -296,8 +296,9 @@ __device__ __forceinline__ void mma_16816(float (&d)[4], const uint32_t (&a)[4],
 }
 
 struct StreamArgs {
-    int64_t nf, nt, ntasks, nobs;
+    int64_t nf, nt, ntasks;
     int64_t task0;      // of blockIdx.y == 0
+    int nobs;           // at most 8 NT
     int nrb, ncb, ngroups;
     int rows;           // row blocks of a CTA
     int per_rank;       // 64-feature blocks to a CTA of the cluster (even)
@@ -330,12 +331,12 @@ __global__ void __launch_bounds__(kStreamThreads, 1)
     q4_stream_kernel(const T* __restrict__ X, const uint4* __restrict__ codes, const T* __restrict__ scales,
                      T* __restrict__ Yhat, StreamArgs a) {
     using H = typename Split16<T>::Type;
-    constexpr int kTerms = Split16<T>::kTerms, kObs = 8 * NT, kSlotFloats = StreamLayout<T, NT>::kSlotFloats;
+    constexpr int kTerms = Split16<T>::kTerms, kSlotFloats = StreamLayout<T, NT>::kSlotFloats;
     extern __shared__ __align__(16) unsigned char smem_raw[];
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, c = lane & 3;
     const int rank = int(blockIdx.x) & ((1 << a.ranks_log2) - 1), ranks = 1 << a.ranks_log2;
-    const int64_t task = a.task0 + blockIdx.y, obs0 = int64_t(blockIdx.z) * kObs;
-    const int obs_here = int(min(int64_t(kObs), a.nobs - obs0));
+    const int64_t task = a.task0 + blockIdx.y;
+    const int obs_here = a.nobs;
     const int rb_begin = (int(blockIdx.x) >> a.ranks_log2) * a.rows, rb_end = min(a.nrb, rb_begin + a.rows);
     const int cb_begin = rank * a.per_rank, cb_end = min(a.ncb, cb_begin + a.per_rank);
     const StreamLayout<T, NT> at(a.chunk, obs_here, min(a.rows, kStreamRows), a.group_shift);
@@ -392,7 +393,7 @@ __global__ void __launch_bounds__(kStreamThreads, 1)
 #pragma unroll 2
                 for (int i = tid; i < obs_here * per_obs; i += kStreamThreads) {
                     const int o = i / per_obs, f = (i - o * per_obs) * kPer;
-                    const T* src = X + ((obs0 + o) * a.ntasks + task) * a.nf + f0 + f;
+                    const T* src = X + (o * a.ntasks + task) * a.nf + f0 + f;
                     T v[kPer] = {};
                     if (a.vec) {
                         if (f < in) VecLoad<T, kPer>::load(src, v);
@@ -511,7 +512,7 @@ __global__ void __launch_bounds__(kStreamThreads, 1)
                     const float* from = slots + (k * kSlots + slot) * kSlotFloats + o * kSlotLd + t % kQ4Rows;
                     v += ranks > 1 ? ld_cluster_f32(from, p) : *from;
                 }
-            if (target < a.nt) Yhat[((obs0 + o) * a.ntasks + task) * a.nt + target] = from_arith<T>(v * kCodeUp<H>);
+            if (target < a.nt) Yhat[(o * a.ntasks + task) * a.nt + target] = from_arith<T>(v * kCodeUp<H>);
         }
         if (ranks > 1) cluster_sync_relaxed();  // the peers have read this CTA's sums
         else if (rb0 + kStreamRows < rb_end) __syncthreads();
@@ -521,14 +522,14 @@ __global__ void __launch_bounds__(kStreamThreads, 1)
 template <typename T, int NT>
 int stream_predict(const T* X, const void* codes, const T* scales, T* Yhat, StreamArgs a, cudaStream_t stream) {
     constexpr size_t kRoom = size_t(224) * 1024;
-    const int obs = int(std::min<int64_t>(8 * NT, a.nobs));
-    const int64_t obs_tiles = (a.nobs + 8 * NT - 1) / (8 * NT), sms = sm_count();
+    const int obs = a.nobs;
+    const int64_t sms = sm_count();
     // CTAs for a task's row blocks, one to an SM
-    const int64_t ctas = std::max<int64_t>(1, sms / std::min(sms, a.ntasks * obs_tiles));
+    const int64_t ctas = std::max<int64_t>(1, sms / std::min(sms, a.ntasks));
     a.rows = int((a.nrb + ctas - 1) / ctas);
     const int64_t groups = (a.nrb + a.rows - 1) / a.rows;
     // CTAs of a cluster: while they find SMs and each warp two blocks of codes
-    while (a.ranks_log2 < 3 && ((groups * a.ntasks * obs_tiles) << (a.ranks_log2 + 1)) <= sms &&
+    while (a.ranks_log2 < 3 && ((groups * a.ntasks) << (a.ranks_log2 + 1)) <= sms &&
            int64_t(a.ncb) * a.rows >= (2 * kStreamWarps) << (a.ranks_log2 + 1))
         ++a.ranks_log2;
     const int ranks = 1 << a.ranks_log2, rows = std::min(a.rows, kStreamRows);
@@ -545,7 +546,6 @@ int stream_predict(const T* X, const void* codes, const T* scales, T* Yhat, Stre
     const auto kernel = kernels[which];
     cudaError_t e = set_smem_limit_once(attr[which], kernel, kRoom);
     if (e != cudaSuccess) return int(e);
-    if (obs_tiles > 65535 || (groups << a.ranks_log2) > 0x7fffffff) return GLMB_ERR_TOO_LARGE;
     cudaLaunchConfig_t cfg = {};
     cfg.blockDim = dim3(kStreamThreads);
     cfg.dynamicSmemBytes = size_t(StreamLayout<T, NT>(a.chunk, obs, rows, a.group_shift).bytes);
@@ -557,8 +557,7 @@ int stream_predict(const T* X, const void* codes, const T* scales, T* Yhat, Stre
     cfg.attrs = at;
     cfg.numAttrs = 1;
     for (a.task0 = 0; a.task0 < a.ntasks; a.task0 += 65535) {
-        cfg.gridDim = dim3(unsigned(groups << a.ranks_log2), unsigned(std::min<int64_t>(65535, a.ntasks - a.task0)),
-                           unsigned(obs_tiles));
+        cfg.gridDim = dim3(unsigned(groups << a.ranks_log2), unsigned(std::min<int64_t>(65535, a.ntasks - a.task0)));
         count_launch();
         e = cudaLaunchKernelEx(&cfg, kernel, X, static_cast<const uint4*>(codes), scales, Yhat, StreamArgs(a));
         if (e != cudaSuccess) return int(e);
@@ -618,7 +617,7 @@ int q4_predict(const T* X, const void* codes, const T* scales, T* Yhat, int64_t 
         return q4_tile_predict<T>(X, codes, scales, Yhat, nf, nt, ntasks, nobs, group, whole_pieces(X, nf, 16), ws,
                                   ws_bytes, stream);
     }
-    StreamArgs a{nf, nt, ntasks, nobs, 0, int(nrb), int(ncb), int(ng), 0, 0, 0, group == 64 ? 0 : 1, 0,
+    StreamArgs a{nf, nt, ntasks, 0, int(nobs), int(nrb), int(ncb), int(ng), 0, 0, 0, group == 64 ? 0 : 1, 0,
                  whole_pieces(X, nf, 16)};
     set_last_path("q4_stream");
     if constexpr (kStreamMost<T> > 8)

@@ -125,7 +125,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     using S = TileShape<T, N>;
     using H = typename Split16<T>::Type;
     constexpr int kStages = S::kStages, kCols = S::kCols, kSub = S::kSub;
-    constexpr uint32_t kTmemCols = N < 32 ? 32 : 2 * N;
+    constexpr uint32_t kTmemCols = 2 * N;
     extern __shared__ __align__(1024) unsigned char smem_raw[];
     TileSmem<T, N>& sm = *reinterpret_cast<TileSmem<T, N>*>(
         reinterpret_cast<unsigned char*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023)));
