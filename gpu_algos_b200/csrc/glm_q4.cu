@@ -90,8 +90,9 @@ __device__ __forceinline__ uint32_t nearest_code(float w, float s, float inv, fl
         const int step = (__float_as_int(d) >> 31) | 1;
         return uint32_t(bits + (fabsf(d) > ((bits & 1) != 0 ? below : half) ? step : 0));
     } else {
-        // One correction makes the quotient the float nearest to w / s, which is w / s itself on a border; of
-        // 16-bit w and s (11 bits at most) any other quotient is 2^-12 of it or more away from one.
+        // One correction by the fused remainder (a Newton step on the quotient, as P. Markstein published it in
+        // 1990) makes it the float nearest to w / s, which is w / s itself on a border; of 16-bit w and s (11 bits
+        // at most) any other quotient is 2^-12 of it or more away from one.
         const float t = w * inv;
         return __float_as_uint(fmaf(fmaf(-t, s, w), inv, t) + kOne);
     }
@@ -269,9 +270,12 @@ __global__ void __launch_bounds__(kThreads)
 // features out over the CTAs of a cluster as well.
 //
 // 16384 x 4096 in groups of 128, bfloat16: 12.1 us for one observation (5.3 us
-// of codes and scales at HBM's copy rate), 16.2 for 8, 21.9 for 16.  About 110
-// instructions per 128 features of a row block, the half of them the codes'
-// unpacking, share the time with the start and the sums at the end (3 to 4 us).
+// of codes and scales at HBM's copy rate), 16.2 for 8, 21.9 for 16.  Not the
+// instructions bound it -- about 110 per 128 features of a row block are 3 us of
+// each scheduler's issue slots, of which 41 % are used -- but latency at both
+// ends: each warp requests its first four pairs of blocks, of some 14 in all,
+// then X and the scales are staged behind a barrier before the first is used,
+// and the slots are summed once the last warp is through.
 // A warp to a row block, its features shared over a cluster of four CTAs, took
 // 18 us: two waves of CTAs, and its index arithmetic as long as its work.
 
@@ -596,9 +600,10 @@ int q4_dequantize(const void* codes, const T* scales, T* M, int64_t nf, int64_t 
     return launch_status();
 }
 
-// Up to this many observations go through the stream kernel.  At 16384 x 4096 both sides took, stream and tile:
-// bfloat16 17.4 and 20.9 us at 9 observations, 21.9 and 20.9 at 16; float, whose three terms take three times the
-// products, 32 and 26.3 us at 9.
+// Up to this many observations go through the stream kernel.  Stream and tile on either side of the limit, in us:
+// bfloat16 at 16 and 17 observations 21.8 and 20.5 on 16384 x 4096, 12.8 and 13.7 on 4096 x 4096, 6.0 and 8.4 on
+// 1000 x 777, 4.7 and 5.2 on 64 models of 16 x 256, 11.8 and 20.7 on 300 of them.  float, whose three terms take
+// three times the products, was measured on both sides at 16384 x 4096 alone, 32 and 26.3 at 9 observations.
 template <typename T>
 constexpr int64_t kStreamMost = sizeof(T) == 2 ? 16 : 8;
 

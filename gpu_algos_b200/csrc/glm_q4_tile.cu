@@ -18,8 +18,10 @@
 // take about 1350: making the operands (two blocks of codes by each warp, 800 to
 // 1000 clocks), draining (640) and issuing the MMAs all run beside each other.
 // At small N an MMA still takes its 256 rows about 85 clocks.  16384 targets x
-// 4096 features, bfloat16: 20.4 us at 17 observations, 24 at 128, 237 at 2048
-// (1.16 PFLOP/s, 0.84 of cuBLAS sustained).  Measured and not kept: the operand
+// 4096 features, bfloat16: 20.4 us at 17 observations, 24 at 128, 231 at 2048
+// while the clock is at 1965 MHz (1.19 PFLOP/s, 0.73 of cuBLAS in a burst); in
+// long runs the power limit holds it to 1.6 GHz, 260 to 270 us (0.75 of cuBLAS
+// sustained).  Measured and not kept: the operand
 // in tensor memory instead of shared memory (it leaves room for N = 192 at
 // most: 408 us against 311 then), two sets of making warps (no gain: the MMA
 // warp is the longest path at small N), four pairs to a cluster (clusters of
